@@ -79,6 +79,72 @@ class mx_qembed_args(C.Structure):
     ]
 
 
+class mx_f8_dense_config(C.Structure):
+    _fields_ = [("activation", C.c_int32), ("weight_layout", C.c_int32), ("output_dtype", C.c_int32)]
+
+
+class mx_f8_quantize_args(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("codes", C.c_void_p),
+        ("scale", C.c_void_p),
+        ("M", C.c_int64),
+        ("K", C.c_int64),
+        ("x_dtype", C.c_int32),
+        ("block_rows", C.c_int32),
+    ]
+
+
+class mx_f8_dense_args(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("x_scale", C.c_void_p),
+        ("w", C.c_void_p),
+        ("w_scale", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("out", C.c_void_p),
+        ("M", C.c_int64),
+        ("K", C.c_int64),
+        ("N", C.c_int64),
+        ("x_dtype", C.c_int32),
+        ("bias_dtype", C.c_int32),
+        ("out_dtype", C.c_int32),
+        ("weight_layout", C.c_int32),
+        ("activation", C.c_int32),
+    ]
+
+
+class mx_f8_weight_grad_args(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("x_scale", C.c_void_p),
+        ("dy", C.c_void_p),
+        ("out", C.c_void_p),
+        ("M", C.c_int64),
+        ("K", C.c_int64),
+        ("N", C.c_int64),
+        ("dy_dtype", C.c_int32),
+        ("out_dtype", C.c_int32),
+        ("weight_layout", C.c_int32),
+    ]
+
+
+class mx_f8_act_grad_args(C.Structure):
+    _fields_ = [
+        ("z", C.c_void_p),
+        ("z_scale", C.c_void_p),
+        ("up", C.c_void_p),
+        ("up_scale", C.c_void_p),
+        ("dy", C.c_void_p),
+        ("dz", C.c_void_p),
+        ("dup", C.c_void_p),
+        ("M", C.c_int64),
+        ("N", C.c_int64),
+        ("dy_dtype", C.c_int32),
+        ("activation", C.c_int32),
+    ]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _I32P = C.POINTER(C.c_int32)
@@ -133,6 +199,10 @@ SIGNATURES = {
     "mx_fn_dot_general": [_P, _VAL, _I32P, _I, _I32P, _I, _VAL, _I32P, _I, _I32P, _I, _I, _I, _VALP],
     "mx_fn_fused_dense": [_P, _VAL, _VAL, _VAL, C.POINTER(mx_dense_config), _VALP],
     "mx_fn_fused_gelu": [_P, _VAL, _I, _VALP],
+    "mx_fn_f8_quantize": [_P, _VAL, _I, _VALP, _VALP],
+    "mx_fn_f8_dense": [_P, _VAL, _VAL, _VAL, _VAL, _VAL, C.POINTER(mx_f8_dense_config), _VALP],
+    "mx_fn_f8_weight_gradient": [_P, _VAL, _VAL, _VAL, _I, _I, _VALP],
+    "mx_fn_f8_activation_gradient": [_P, _VAL, _VAL, _VAL, _VAL, _VAL, _I, _VALP, _VALP],
     "mx_fn_unary": [_P, _I, _VAL, _VALP],
     "mx_fn_binary": [_P, _I, _VAL, _VAL, _VALP],
     "mx_fn_convert_dtype": [_P, _VAL, _I, _VALP],
@@ -155,6 +225,12 @@ SIGNATURES = {
     "mx_qdense_plan": [_P, C.POINTER(mx_qdense_args), C.c_char_p, _SZ],
     "mx_qdense_noalloc": [_P, C.POINTER(mx_qdense_args)],
     "mx_quantized_embedding_lookup": [_P, C.POINTER(mx_qembed_args)],
+    "mx_f8_quantize": [_P, C.POINTER(mx_f8_quantize_args)],
+    "mx_f8_dense": [_P, C.POINTER(mx_f8_dense_args)],
+    "mx_f8_dense_plan": [_P, C.POINTER(mx_f8_dense_args), C.c_char_p, _SZ],
+    "mx_f8_weight_gradient": [_P, C.POINTER(mx_f8_weight_grad_args)],
+    "mx_f8_weight_gradient_plan": [_P, C.POINTER(mx_f8_weight_grad_args), C.c_char_p, _SZ],
+    "mx_f8_activation_gradient": [_P, C.POINTER(mx_f8_act_grad_args)],
 }
 
 _RESTYPES = {"mx_last_error": C.c_char_p}

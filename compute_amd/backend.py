@@ -118,6 +118,11 @@ class OpType(enum.IntEnum):
     FusedScaledDotProductAttention = 120
     FusedQuantizedDense = 123
     QuantizedEmbeddingLookup = 124
+    # Operators on 8-bit floating-point blocks (no counterpart in the reference's enum).
+    F8Quantize = 1000
+    F8Dense = 1001
+    F8WeightGradient = 1002
+    F8ActivationGradient = 1003
 
 
 NF4LookupTable = np.array([
@@ -193,6 +198,18 @@ class DenseConfig:
     WeightLayout: DenseLayout = DenseLayoutInputOutputs
 
 
+F8Block = 128  # values of a row per scale of the F8 operators; weights have one per 128 x 128 block
+
+
+@dataclass
+class F8DenseConfig:
+    """mx_f8_dense_config: OutputDType Float32 or BFloat16 (InvalidDType: x's, BFloat16 for codes)."""
+
+    Activation: ActivationType = ActivationNone
+    WeightLayout: DenseLayout = DenseLayoutInputOutputs
+    OutputDType: DType = DType.InvalidDType
+
+
 @dataclass
 class DotGeneralConfig:
     """compute.DotGeneralConfig (standard_ops.go:91-111)."""
@@ -245,7 +262,7 @@ def _host_bytes(flat: Any, shape: Shape) -> np.ndarray:
     want = shape.dtype.numpy_storage()
     arr = np.ascontiguousarray(np.asarray(flat))
     if arr.dtype != want:
-        if shape.dtype in (DType.BFloat16, DType.Int4, DType.Uint4) and arr.dtype.kind == "f":
+        if shape.dtype in (DType.BFloat16, DType.Int4, DType.Uint4, DType.F8E4M3FN) and arr.dtype.kind == "f":
             raise ComputeError(_lib.MX_ERR_INVALID,
                                f"{shape.dtype} data must be given as {want} storage, got {arr.dtype}")
         arr = arr.astype(want)
@@ -348,6 +365,29 @@ class Backend:
 
     def QEmbed(self, args: _lib.mx_qembed_args) -> None:
         _check(self._lib.mx_quantized_embedding_lookup(self._h, C.byref(args)))
+
+    # -- operators on 8-bit floating-point blocks (device pointers, the backend's stream) --------
+    def F8Quantize(self, args: _lib.mx_f8_quantize_args) -> None:
+        _check(self._lib.mx_f8_quantize(self._h, C.byref(args)))
+
+    def F8Dense(self, args: _lib.mx_f8_dense_args) -> None:
+        _check(self._lib.mx_f8_dense(self._h, C.byref(args)))
+
+    def F8DensePlan(self, args: _lib.mx_f8_dense_args) -> str:
+        buf = C.create_string_buffer(128)
+        _check(self._lib.mx_f8_dense_plan(self._h, C.byref(args), buf, len(buf)))
+        return buf.value.decode()
+
+    def F8WeightGradient(self, args: _lib.mx_f8_weight_grad_args) -> None:
+        _check(self._lib.mx_f8_weight_gradient(self._h, C.byref(args)))
+
+    def F8WeightGradientPlan(self, args: _lib.mx_f8_weight_grad_args) -> str:
+        buf = C.create_string_buffer(128)
+        _check(self._lib.mx_f8_weight_gradient_plan(self._h, C.byref(args), buf, len(buf)))
+        return buf.value.decode()
+
+    def F8ActivationGradient(self, args: _lib.mx_f8_act_grad_args) -> None:
+        _check(self._lib.mx_f8_activation_gradient(self._h, C.byref(args)))
 
     # -- profiling / debugging ------------------------------------------------------------
     def SetProfiling(self, enabled: bool) -> None:
@@ -578,6 +618,34 @@ class Function:
 
     def FusedGelu(self, x: Value, exact: bool) -> Value:
         return self._out(self._lib.mx_fn_fused_gelu, int(x), int(bool(exact)))
+
+    # -- operators on 8-bit floating-point blocks -------------------------------------------
+    def FusedF8Quantize(self, x: Value, blockRows: int = 1) -> tuple:
+        """(codes, scale) of x: one scale per 128 values of a row, or (blockRows 128) per 128 x 128 block."""
+        codes, scale = C.c_uint64(), C.c_uint64()
+        _check(self._lib.mx_fn_f8_quantize(self._h, int(x), int(blockRows), C.byref(codes), C.byref(scale)))
+        return Value(codes.value), Value(scale.value)
+
+    def FusedF8Dense(self, x: Value, xScale: Optional[Value], weight: Value, weightScale: Value, bias: Optional[Value],
+                     options: Optional[F8DenseConfig] = None) -> Value:
+        """act(x W + bias); x codes with xScale, or float values (xScale None) that are quantised first."""
+        o = options if options is not None else F8DenseConfig()
+        cfg = _lib.mx_f8_dense_config(int(o.Activation), int(o.WeightLayout), int(o.OutputDType))
+        return self._out(self._lib.mx_fn_f8_dense, int(x), int(xScale or 0), int(weight), int(weightScale), int(bias or 0),
+                         C.byref(cfg))
+
+    def FusedF8WeightGradient(self, x: Value, xScale: Value, dy: Value, weightLayout: DenseLayout = DenseLayoutInputOutputs,
+                              outputDType: DType = DType.InvalidDType) -> Value:
+        """x^T dy [K, N] (or its transpose [N, K]) of x kept in 8 bits."""
+        return self._out(self._lib.mx_fn_f8_weight_gradient, int(x), int(xScale), int(dy), int(weightLayout), int(outputDType))
+
+    def FusedF8ActivationGradient(self, z: Value, zScale: Value, dy: Value, activation: ActivationType,
+                                  up: Optional[Value] = None, upScale: Optional[Value] = None):
+        """dy * act'(z) of z kept in 8 bits; with up (the gated product act(z) * up) the pair (dz, dup)."""
+        dz, dup = C.c_uint64(), C.c_uint64()
+        _check(self._lib.mx_fn_f8_activation_gradient(self._h, int(z), int(zScale), int(up or 0), int(upScale or 0), int(dy),
+                                                      int(activation), C.byref(dz), C.byref(dup) if up else None))
+        return (Value(dz.value), Value(dup.value)) if up else Value(dz.value)
 
     # -- standard ops ---------------------------------------------------------------------
     def DotGeneral(self, lhs: Value, lhsContractingAxes, lhsBatchAxes, rhs: Value, rhsContractingAxes,

@@ -1,0 +1,85 @@
+// Device helpers of the operators on 8-bit floating-point blocks: e4m3 codes with one float32 scale
+// for every 128 consecutive values of a row, or for every 128 x 128 block of a weight matrix.
+#pragma once
+
+#include <type_traits>
+
+#include "device_common.h"
+
+namespace mx {
+namespace f8 {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
+
+constexpr int kBlock = MX_F8_BLOCK;
+
+inline int64_t blocks(int64_t n) { return (n + kBlock - 1) / kBlock; }
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// 32 consecutive codes, an operand of the 16x16x128 MFMA, from 16-byte aligned memory.
+__device__ __forceinline__ i32x8 join(const u32x4& lo, const u32x4& hi) {
+  return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+__device__ __forceinline__ i32x8 read32(const uint8_t* p) { return join(*(const u32x4*)p, *(const u32x4*)(p + 16)); }
+
+// The four values of a word of codes (v_cvt_pk_f32_fp8: exact, NaN codes to NaN).
+__device__ __forceinline__ f32x4 decode4(uint32_t w) {
+  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  return f32x4{a.x, a.y, b.x, b.y};
+}
+
+// Eight codes as the bf16 values they stand for (exact), an operand of the bf16 16x16x32 MFMA.
+__device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Four values, at most 448 in magnitude, to codes (round to nearest even; NaN to a NaN code).
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+
+// The magnitude bits of a finite value, 0 of an infinity or NaN: they compare as integers.
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
+  return u < 0x7f800000u ? u : 0u;
+}
+
+// The exponent of a block's scale from its largest magnitude's bits: the smallest e >= -126 with
+// a <= 448 * 2^e.  a = 1.f * 2^(E - 127) and 448 = 1.75 * 2^8, so e = E - 135, and one more where
+// 1.f > 1.75.  0 (a scale of 1) where a is 0.  At most 120, so that 2^e and 2^-e are normal floats.
+__device__ __forceinline__ int scale_exponent(uint32_t a) {
+  const int e = (int)(a >> 23) - 135 + ((a & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return a == 0 ? 0 : max(e, -126);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// v / s for s = 2^-e as v * inv, exact (or below any code); NaN where v is not finite, as the format
+// holds no infinity.
+__device__ __forceinline__ float scaled(float v, float inv) {
+  return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : v * inv;
+}
+
+// The largest of 16 lanes' values (a row of the wave), in every lane of the row.
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+  auto step = [&](auto ctrl) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xf, 0xf, true);
+    v = v > o ? v : o;
+  };
+  step(std::integral_constant<int, 0xB1>{});   // quad_perm 1,0,3,2
+  step(std::integral_constant<int, 0x4E>{});   // quad_perm 2,3,0,1
+  step(std::integral_constant<int, 0x141>{});  // row_half_mirror
+  step(std::integral_constant<int, 0x140>{});  // row_mirror
+  return v;
+}
+
+}  // namespace f8
+}  // namespace mx

@@ -1,0 +1,149 @@
+// Dense product over 8-bit floating-point blocks:
+//   y[m, n] = act(sum_b sx[m, b] * sw[b, n / 128] * (sum_{k in block b} x[m, k] * w[k, n]) + bias[n]).
+//
+// A block of 128 codes is one v_mfma_f32_16x16x128_f8f6f4, whose sum starts from zero and enters the
+// float32 total with the block's two scales: acc += t * (sx * sw).
+//
+// Precision.  The matrix cores add the products of 8-bit operands in groups of eight, aligned to the
+// group's largest and cut off 13 bits below it (measured with single products, for every 8-bit form
+// of the instruction); groups are added in float32.  On random codes of mixed exponents a sum of 128
+// is 4.4e-5 off in norm.  That is 1/38 of the rounding of a bfloat16 result, which therefore takes
+// these instructions at 4.4 PFLOP/s.  A float32 result (WIDE) takes the codes as bfloat16 values, which
+// are exact, through v_mfma_f32_16x16x32_bf16, whose sums are good to 2^-23 of their terms, at half the
+// rate.
+//
+// Operand layout.  Lane (i = lane % 16, g = lane / 16) of the instruction holds 32 consecutive codes of
+// row (or column) i, those from 32 g; the sum does not depend on which k a position stands for as
+// long as both operands agree.  WIDE: four instructions, each over eight of a lane's 32 codes.  The
+// result: column i, rows 4 g .. 4 g + 3.
+#include <algorithm>
+
+#include "f8_common.h"
+#include "mxrt_internal.h"
+
+namespace mx {
+namespace {
+using namespace f8;
+
+struct DenseArgs {
+  const uint8_t* x;
+  const float* x_scale;
+  const uint8_t* w;
+  const float* w_scale;
+  const void* bias;
+  void* out;
+  int M, K, N, KB, NB;
+  int b_dt, out_dt, act, oi;
+  int tiles_n;
+};
+
+__device__ __forceinline__ f32x4 mfma_f8(const i32x8& a, const i32x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+}
+
+// The sum of products of one block.
+template <bool WIDE>
+__device__ __forceinline__ f32x4 block_sum(const i32x8& a, const i32x8& b) {
+  f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8((uint32_t)a[2 * j], (uint32_t)a[2 * j + 1]),
+                                                  widen8((uint32_t)b[2 * j], (uint32_t)b[2 * j + 1]), t, 0, 0, 0);
+    return t;
+  } else {
+    return mfma_f8(a, b, t);
+  }
+}
+
+// 16 bytes from p, of which the first n are in the row (the rest 0).  Rows may start at any byte.
+__device__ __forceinline__ u32x4 load16(const uint8_t* p, int n) {
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (n >= 16) {
+    __builtin_memcpy(&v, p, 16);
+  } else {
+    for (int i = 0; i < n; ++i) v[i / 4] |= (uint32_t)p[i] << (8 * (i % 4));
+  }
+  return v;
+}
+
+// Any sizes, alignment and layout: 64 x 64 tiles, both operands staged in LDS as rows of 128 codes.
+constexpr int kAnyTile = 64, kAnyThreads = 256, kAnyPitch = kBlock + 16;
+
+template <bool WIDE>
+__global__ __launch_bounds__(kAnyThreads) void f8_dense_any_kernel(DenseArgs a) {
+  __shared__ __align__(16) uint8_t xs[kAnyTile * kAnyPitch], ws[kAnyTile * kAnyPitch];
+  const int m0 = (int)(blockIdx.x / (unsigned)a.tiles_n) * kAnyTile, n0 = (int)(blockIdx.x % (unsigned)a.tiles_n) * kAnyTile;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, i = lane % 16, g = lane / 16;
+  f32x4 acc[4] = {};
+  for (int kb = 0; kb < a.KB; ++kb) {
+    const int k0 = kb * kBlock;
+    __syncthreads();
+    for (int c = threadIdx.x; c < kAnyTile * 8; c += kAnyThreads) {
+      const int r = c / 8, k = k0 + 16 * (c % 8);
+      const bool in = m0 + r < a.M;
+      *(u32x4*)(xs + r * kAnyPitch + 16 * (c % 8)) = load16(a.x + (in ? (int64_t)(m0 + r) * a.K + k : 0), in ? a.K - k : 0);
+    }
+    if (a.oi) {
+      for (int c = threadIdx.x; c < kAnyTile * 8; c += kAnyThreads) {
+        const int r = c / 8, k = k0 + 16 * (c % 8);
+        const bool in = n0 + r < a.N;
+        *(u32x4*)(ws + r * kAnyPitch + 16 * (c % 8)) = load16(a.w + (in ? (int64_t)(n0 + r) * a.K + k : 0), in ? a.K - k : 0);
+      }
+    } else {
+      for (int c = threadIdx.x; c < kBlock * 4; c += kAnyThreads) {
+        const int r = c / 4, n = n0 + 16 * (c % 4);
+        const bool in = k0 + r < a.K;
+        const u32x4 v = load16(a.w + (in ? (int64_t)(k0 + r) * a.N + n : 0), in ? a.N - n : 0);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) ws[(16 * (c % 4) + j) * kAnyPitch + r] = (uint8_t)(v[j / 4] >> (8 * (j % 4)));
+      }
+    }
+    __syncthreads();
+    float sx[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int m = m0 + 16 * wave + 4 * g + r;
+      sx[r] = m < a.M ? a.x_scale[(int64_t)m * a.KB + kb] : 0.0f;
+    }
+    const float sw = a.oi ? a.w_scale[(int64_t)(n0 / kBlock) * a.KB + kb] : a.w_scale[(int64_t)kb * a.NB + n0 / kBlock];
+    const i32x8 xa = read32(xs + (16 * wave + i) * kAnyPitch + 32 * g);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const i32x8 wb = read32(ws + (16 * c + i) * kAnyPitch + 32 * g);
+      const f32x4 t = block_sum<WIDE>(xa, wb);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[c][r] = fmaf(t[r], sx[r] * sw, acc[c][r]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int n = n0 + 16 * c + i;
+    if (n >= a.N) continue;
+    const float bias = a.bias ? load_f(a.bias, n, a.b_dt) : 0.0f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int m = m0 + 16 * wave + 4 * g + r;
+      if (m < a.M) store_f(a.out, (int64_t)m * a.N + n, a.out_dt, act_fast(acc[c][r] + bias, a.act));
+    }
+  }
+}
+
+}  // namespace
+
+const char* f8_product_name(const F8DenseDesc&) { return "f8_dense_any"; }
+
+int f8_product_run(mx_backend* b, const F8DenseDesc& d) {
+  if (d.M == 0 || d.N == 0) return MX_OK;
+  DenseArgs a{(const uint8_t*)d.x, d.x_scale, d.w, d.w_scale, d.bias, d.out, (int)d.M, (int)d.K, (int)d.N, (int)blocks(d.K),
+              (int)blocks(d.N), d.b_dt, d.out_dt, d.act, d.oi, 0};
+  const int64_t tm = (d.M + kAnyTile - 1) / kAnyTile, tn = (d.N + kAnyTile - 1) / kAnyTile;
+  if (tm * tn >= (int64_t)1 << 31) return set_error(MX_ERR_INVALID, "F8Dense: more than 2^31 workgroups");
+  a.tiles_n = (int)tn;
+  auto k = d.out_dt == MX_DTYPE_FLOAT32 ? f8_dense_any_kernel<true> : f8_dense_any_kernel<false>;
+  return launch(b, f8_product_name(d), [&] {
+    dispatch(k, dim3((unsigned)(tm * tn)), dim3(kAnyThreads), 0, b->stream, a);
+  });
+}
+
+}  // namespace mx

@@ -1,0 +1,290 @@
+// Quantisation into 8-bit floating-point blocks, and the gradient of an activation from its input
+// kept in that form.  Both are one pass over their data and bound by HBM.
+//
+// Quantisation.  With a the largest finite magnitude of a block, its scale s is the smallest power of
+// two with a <= 448 s and a code is x / s rounded to nearest even.  A power of two costs nothing in a
+// floating format (a code keeps its four significant bits wherever it lies in the range; the block's
+// smallest values lose one binade of about 17), the division is exact, so every implementation of the
+// definition gives the same codes, and a value read back, code * s, is exact in bf16.
+//
+// A row of 16 lanes holds a block of 128 values, eight a lane (one 16-byte load of bf16, two of f32,
+// one 8-byte store of codes), so that the maximum of a block takes four DPP steps and no LDS.
+//
+// Activation gradient.  z' = dy * act'(z) (and, gated, dy * up * act'(z) and dy * act(z)) with z and up
+// decoded from their codes: 1 or 2 bytes of codes, dy and one or two results per value.  A lane takes
+// eight consecutive values, which share a scale.
+#include <algorithm>
+
+#include "f8_common.h"
+#include "mxrt_internal.h"
+
+namespace mx {
+namespace {
+using namespace f8;
+
+constexpr int kThreads = 256;
+constexpr int kPerLane = 8;                        // values of a lane
+constexpr int kLanes = kBlock / kPerLane;          // lanes of a block: a DPP row
+constexpr int kGroups = kThreads / kLanes;         // blocks of a workgroup
+
+// Eight consecutive values from element `at`, of which the first n are in the row; the rest 0.
+// VEC: rows and array start on 16 bytes, so all eight are in the row or none.
+template <bool F32, bool VEC>
+__device__ __forceinline__ void load8(const void* p, int64_t at, int n, float (&v)[8]) {
+  if constexpr (VEC) {
+    if (n > 0) {
+      if constexpr (F32) {
+        const f32x4* q = (const f32x4*)((const float*)p + at);
+        const f32x4 a = q[0], b = q[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+      } else {
+        const u32x4 a = *(const u32x4*)((const uint16_t*)p + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(a[i] << 16), v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = i < n ? (F32 ? ((const float*)p)[at + i] : bf16_to_f32(((const uint16_t*)p)[at + i])) : 0.0f;
+  }
+}
+
+template <bool F32, bool VEC>
+__device__ __forceinline__ void store8(void* p, int64_t at, int n, const float (&v)[8]) {
+  if constexpr (VEC) {
+    if (n > 0) {
+      if constexpr (F32) {
+        f32x4* q = (f32x4*)((float*)p + at);
+        q[0] = f32x4{v[0], v[1], v[2], v[3]};
+        q[1] = f32x4{v[4], v[5], v[6], v[7]};
+      } else {
+        u32x4 o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = (uint32_t)f32_to_bf16(v[2 * i]) | (uint32_t)f32_to_bf16(v[2 * i + 1]) << 16;
+        *(u32x4*)((uint16_t*)p + at) = o;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) {
+        if constexpr (F32)
+          ((float*)p)[at + i] = v[i];
+        else
+          ((uint16_t*)p)[at + i] = f32_to_bf16(v[i]);
+      }
+  }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_codes8(uint8_t* p, int64_t at, int n, const float (&v)[8], float inv) {
+  const u32x2 c = {encode4(scaled(v[0], inv), scaled(v[1], inv), scaled(v[2], inv), scaled(v[3], inv)),
+                   encode4(scaled(v[4], inv), scaled(v[5], inv), scaled(v[6], inv), scaled(v[7], inv))};
+  if constexpr (VEC) {
+    if (n > 0) *(u32x2*)(p + at) = c;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[at + i] = (uint8_t)(c[i / 4] >> (8 * (i % 4)));
+  }
+}
+
+__device__ __forceinline__ uint32_t largest8(const float (&v)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, finite_bits(v[i]));
+  return m;
+}
+
+// One scale per 128 values of a row: block t of the M * KB blocks is row t / KB's.
+template <bool F32, bool VEC>
+__global__ __launch_bounds__(kThreads) void f8_quantize_rows_kernel(const void* x, uint8_t* codes, float* scale, int K,
+                                                                    int KB, int64_t total) {
+  const int64_t t = (int64_t)blockIdx.x * kGroups + threadIdx.x / kLanes;
+  if (t >= total) return;
+  const int64_t row = t / KB;
+  const int k0 = (int)(t - row * KB) * kBlock + (int)(threadIdx.x % kLanes) * kPerLane;
+  const int n = K - k0;
+  const int64_t at = row * K + k0;
+  float v[8];
+  load8<F32, VEC>(x, at, n, v);
+  const int e = scale_exponent(row_max(largest8(v)));
+  store_codes8<VEC>(codes, at, n, v, pow2(-e));
+  if (threadIdx.x % kLanes == 0) scale[t] = pow2(e);
+}
+
+// One scale per 128 x 128 block: a workgroup's, its values held in registers between the passes.
+template <bool F32, bool VEC>
+__global__ __launch_bounds__(kThreads) void f8_quantize_tiles_kernel(const void* x, uint8_t* codes, float* scale, int M,
+                                                                     int K, int KB) {
+  constexpr int kPasses = kBlock / kGroups;
+  __shared__ uint32_t part[kThreads / 64];
+  const int rb = (int)(blockIdx.x / (unsigned)KB), cb = (int)(blockIdx.x % (unsigned)KB);
+  const int k0 = cb * kBlock + (int)(threadIdx.x % kLanes) * kPerLane;
+  const int n = K - k0;
+  float v[kPasses][8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int row = rb * kBlock + p * kGroups + (int)(threadIdx.x / kLanes);
+    load8<F32, VEC>(x, (int64_t)row * K + k0, row < M ? n : 0, v[p]);
+  }
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) m = max(m, largest8(v[p]));
+  m = row_max(m);
+  m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+  m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+  if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = m;
+  __syncthreads();
+  for (int i = 0; i < kThreads / 64; ++i) m = max(m, part[i]);
+  const int e = scale_exponent(m);
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int row = rb * kBlock + p * kGroups + (int)(threadIdx.x / kLanes);
+    store_codes8<VEC>(codes, (int64_t)row * K + k0, row < M ? n : 0, v[p], pow2(-e));
+  }
+  if (threadIdx.x == 0) scale[(int64_t)rb * KB + cb] = pow2(e);
+}
+
+// act(z) and its slope.  The values are those of f32 formulas on OCML's erf, exp and tanh.
+template <int ACT>
+__device__ __forceinline__ void act_and_slope(float z, float& a, float& s) {
+  if constexpr (ACT == MX_ACT_GELU) {
+    const float cdf = 0.5f * erfcf(-0.70710678118654752f * z);
+    a = z * cdf;
+    s = fmaf(z * 0.39894228040143268f, __expf(-0.5f * z * z), cdf);
+  } else if constexpr (ACT == MX_ACT_RELU) {
+    a = z < 0.0f ? 0.0f : z;
+    s = z > 0.0f ? 1.0f : z == z ? 0.0f : z;
+  } else if constexpr (ACT == MX_ACT_SILU) {
+    const float g = 1.0f / (1.0f + __expf(-z));
+    a = z * g;
+    s = g * fmaf(z, 1.0f - g, 1.0f);
+  } else if constexpr (ACT == MX_ACT_HARDSWISH) {
+    float v = z * (1.0f / 6.0f) + 0.5f;
+    v = v > 0.0f ? v : v == v ? 0.0f : v;
+    v = v < 1.0f ? v : v == v ? 1.0f : v;
+    a = z * v;
+    s = z <= -3.0f ? 0.0f : z >= 3.0f ? 1.0f : fmaf(z, 1.0f / 3.0f, 0.5f);
+  } else if constexpr (ACT == MX_ACT_TANH) {
+    a = tanhf(z);
+    // 1 - tanh^2 = 4 e / (1 + e)^2 with e = exp(-2 |z|), without the cancellation
+    const float e = __expf(-2.0f * fabsf(z)), d = 1.0f / (1.0f + e);
+    s = 4.0f * e * d * d;
+  } else {
+    a = z;
+    s = 1.0f;
+  }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void load_codes8(const uint8_t* p, int64_t at, int n, float scale, float (&v)[8]) {
+  u32x2 c = {0u, 0u};
+  if constexpr (VEC) {
+    if (n > 0) c = *(const u32x2*)(p + at);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) c[i / 4] |= (uint32_t)p[at + i] << (8 * (i % 4));
+  }
+  const f32x4 a = decode4(c.x), b = decode4(c.y);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = a[i] * scale, v[4 + i] = b[i] * scale;
+}
+
+struct ActGradArgs {
+  const uint8_t *z, *up;
+  const float *z_scale, *up_scale;
+  const void* dy;
+  void *dz, *dup;
+  int N, NB;
+  int64_t total;  // blocks
+};
+
+template <bool F32, bool VEC, bool GATED, int ACT>
+__global__ __launch_bounds__(kThreads) void f8_act_grad_kernel(ActGradArgs a) {
+  const int64_t t = (int64_t)blockIdx.x * kGroups + threadIdx.x / kLanes;
+  if (t >= a.total) return;
+  const int64_t row = t / a.NB;
+  const int n0 = (int)(t - row * a.NB) * kBlock + (int)(threadIdx.x % kLanes) * kPerLane;
+  const int n = a.N - n0;
+  const int64_t at = row * a.N + n0;
+  float z[8], up[8], dy[8], dz[8], dup[8];
+  load_codes8<VEC>(a.z, at, n, a.z_scale[t], z);
+  if constexpr (GATED) load_codes8<VEC>(a.up, at, n, a.up_scale[t], up);
+  load8<F32, VEC>(a.dy, at, n, dy);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float act, slope;
+    act_and_slope<ACT>(z[i], act, slope);
+    dz[i] = (GATED ? dy[i] * up[i] : dy[i]) * slope;
+    dup[i] = dy[i] * act;
+  }
+  store8<F32, VEC>(a.dz, at, n, dz);
+  if constexpr (GATED) store8<F32, VEC>(a.dup, at, n, dup);
+}
+
+template <bool F32, bool VEC, bool GATED>
+auto act_grad_kernel(int act) {
+  switch (act) {
+    case MX_ACT_GELU: return f8_act_grad_kernel<F32, VEC, GATED, MX_ACT_GELU>;
+    case MX_ACT_RELU: return f8_act_grad_kernel<F32, VEC, GATED, MX_ACT_RELU>;
+    case MX_ACT_SILU: return f8_act_grad_kernel<F32, VEC, GATED, MX_ACT_SILU>;
+    case MX_ACT_HARDSWISH: return f8_act_grad_kernel<F32, VEC, GATED, MX_ACT_HARDSWISH>;
+    case MX_ACT_TANH: return f8_act_grad_kernel<F32, VEC, GATED, MX_ACT_TANH>;
+    default: return f8_act_grad_kernel<F32, VEC, GATED, MX_ACT_NONE>;
+  }
+}
+
+int grid_too_large(const char* op) { return set_error(MX_ERR_INVALID, "%s: more than 2^31 workgroups", op); }
+constexpr int64_t kMaxGrid = ((int64_t)1 << 31) - 1;
+
+bool aligned8(const void* p) { return ((uintptr_t)p & 7) == 0; }
+
+}  // namespace
+
+int f8_quantize_run(mx_backend* b, const F8QuantizeDesc& d) {
+  if (d.M == 0 || d.K == 0) return MX_OK;
+  const bool f32 = d.x_dt == MX_DTYPE_FLOAT32;
+  const bool vec = d.K % kPerLane == 0 && aligned16(d.x) && aligned8(d.codes);
+  const int64_t KB = blocks(d.K);
+  if (d.rows == 1) {
+    const int64_t total = d.M * KB, grid = (total + kGroups - 1) / kGroups;
+    if (grid > kMaxGrid) return grid_too_large("F8Quantize");
+    auto k = f32 ? (vec ? f8_quantize_rows_kernel<true, true> : f8_quantize_rows_kernel<true, false>)
+                 : (vec ? f8_quantize_rows_kernel<false, true> : f8_quantize_rows_kernel<false, false>);
+    return launch(b, "f8_quantize_rows", [&] {
+      dispatch(k, dim3((unsigned)grid), dim3(kThreads), 0, b->stream, d.x, d.codes, d.scale, (int)d.K, (int)KB, total);
+    });
+  }
+  const int64_t grid = blocks(d.M) * KB;
+  if (grid > kMaxGrid) return grid_too_large("F8Quantize");
+  auto k = f32 ? (vec ? f8_quantize_tiles_kernel<true, true> : f8_quantize_tiles_kernel<true, false>)
+               : (vec ? f8_quantize_tiles_kernel<false, true> : f8_quantize_tiles_kernel<false, false>);
+  return launch(b, "f8_quantize_tiles", [&] {
+    dispatch(k, dim3((unsigned)grid), dim3(kThreads), 0, b->stream, d.x, d.codes, d.scale, (int)d.M, (int)d.K, (int)KB);
+  });
+}
+
+int f8_act_grad_run(mx_backend* b, const F8ActGradDesc& d) {
+  if (d.M == 0 || d.N == 0) return MX_OK;
+  const bool f32 = d.dy_dt == MX_DTYPE_FLOAT32, gated = d.up != nullptr;
+  const bool vec = d.N % kPerLane == 0 && aligned8(d.z) && aligned8(d.up) && aligned16(d.dy) && aligned16(d.dz) && aligned16(d.dup);
+  const int64_t NB = blocks(d.N), total = d.M * NB, grid = (total + kGroups - 1) / kGroups;
+  if (grid > kMaxGrid) return grid_too_large("F8ActivationGradient");
+  const ActGradArgs a{d.z, d.up, d.z_scale, d.up_scale, d.dy, d.dz, d.dup, (int)d.N, (int)NB, total};
+  auto k = f32 ? (vec ? (gated ? act_grad_kernel<true, true, true>(d.act) : act_grad_kernel<true, true, false>(d.act))
+                      : (gated ? act_grad_kernel<true, false, true>(d.act) : act_grad_kernel<true, false, false>(d.act)))
+               : (vec ? (gated ? act_grad_kernel<false, true, true>(d.act) : act_grad_kernel<false, true, false>(d.act))
+                      : (gated ? act_grad_kernel<false, false, true>(d.act) : act_grad_kernel<false, false, false>(d.act)));
+  return launch(b, gated ? "f8_act_grad_gated" : "f8_act_grad", [&] {
+    dispatch(k, dim3((unsigned)grid), dim3(kThreads), 0, b->stream, a);
+  });
+}
+
+}  // namespace mx

@@ -42,6 +42,11 @@ enum class Op {
   kCopy,
   kRmsNorm,
   kQEmbed,  // fused row RMS normalisation (compile-time fusion)
+  kSecondOutput,  // storage of the next node's second output, which that node writes (its last input)
+  kF8Quantize,
+  kF8Dense,
+  kF8WGrad,
+  kF8ActGrad,
 };
 
 static const char* op_name(Op op) {
@@ -63,6 +68,11 @@ static const char* op_name(Op op) {
     case Op::kCopy: return "Copy";
     case Op::kRmsNorm: return "RmsNorm";
     case Op::kQEmbed: return "QuantizedEmbeddingLookup";
+    case Op::kSecondOutput: return "SecondOutput";
+    case Op::kF8Quantize: return "FusedF8Quantize";
+    case Op::kF8Dense: return "FusedF8Dense";
+    case Op::kF8WGrad: return "FusedF8WeightGradient";
+    case Op::kF8ActGrad: return "FusedF8ActivationGradient";
   }
   return "?";
 }
@@ -91,6 +101,9 @@ struct Node {
   // DotNorm.
   int64_t B = 0;
   bool rhs_t = false;
+  // F8 operators: rows per scale block, weights [out, in], x in codes, the last input is a second output.
+  int rows = 0;
+  bool oi = false, has_xs = false, second = false;
   // Gather / broadcast / reduce / iota.
   std::vector<int64_t> strides;
   std::vector<int64_t> in_dims;  // reduce: operand dims; binary: lhs dims
@@ -269,6 +282,7 @@ static bool supported_op(int op) {
     case MX_OP_REDUCE_SUM: case MX_OP_RESHAPE: case MX_OP_RSQRT: case MX_OP_SLICE: case MX_OP_SQRT:
     case MX_OP_SUB: case MX_OP_TANH: case MX_OP_TRANSPOSE: case MX_OP_FUSED_GELU: case MX_OP_FUSED_DENSE:
     case MX_OP_FUSED_QUANTIZED_DENSE: case MX_OP_QUANTIZED_EMBEDDING_LOOKUP:
+    case MX_OP_F8_QUANTIZE: case MX_OP_F8_DENSE: case MX_OP_F8_WEIGHT_GRADIENT: case MX_OP_F8_ACTIVATION_GRADIENT:
       return true;
     default:
       return false;
@@ -831,6 +845,213 @@ int mx_fn_fused_gelu(mx_function* fn, mx_value xv, int exact, mx_value* out) {
 }
 
 // ---------------------------------------------------------------------------------------------
+// Operators on 8-bit floating-point blocks.
+// ---------------------------------------------------------------------------------------------
+static int64_t f8_blocks(int64_t n) { return (n + MX_F8_BLOCK - 1) / MX_F8_BLOCK; }
+static bool f32_or_bf16(int dt) { return dt == MX_DTYPE_FLOAT32 || dt == MX_DTYPE_BFLOAT16; }
+
+// Codes [batch..., K] with scales [batch..., ceil(K/128)]; *rows: the product of the leading dims.
+static int f8_check_rows(const char* op, const char* what, const Shape& c, const Shape& s, int64_t* rows) {
+  if (c.dtype != MX_DTYPE_F8E4M3FN)
+    return set_error(MX_ERR_NOT_IMPLEMENTED, "%s: %s must be F8E4M3FN, got %s", op, what, dtype_name(c.dtype));
+  if (c.rank() < 1) return set_error(MX_ERR_INVALID, "%s: %s must have rank >= 1, got %d", op, what, c.rank());
+  Shape want = c;
+  want.dtype = MX_DTYPE_FLOAT32;
+  want.dims.back() = f8_blocks(c.dims.back());
+  if (s != want)
+    return set_error(MX_ERR_INVALID, "%s: scales of %s must be %s, got %s", op, what, want.str().c_str(), s.str().c_str());
+  *rows = 1;
+  for (int i = 0; i + 1 < c.rank(); ++i) *rows *= c.dims[i];
+  return MX_OK;
+}
+
+// Dimensions that the kernels index with 32 bits, past the last by up to a tile.
+static int f8_check_sizes(const char* op, int64_t M, int64_t K, int64_t N) {
+  if (M >= (int64_t)1 << 30 || K >= (int64_t)1 << 30 || N >= (int64_t)1 << 30)
+    return set_error(MX_ERR_INVALID, "%s: rows and columns must be < 2^30", op);
+  return MX_OK;
+}
+
+// Adds the storage node of a second output and then the node that writes it.
+static int add_two_outputs(mx_function* fn, Node n, const Shape& second, mx_value* out, mx_value* out2) {
+  Node st;
+  st.op = Op::kSecondOutput;
+  st.shape = second;
+  MX_TRY(add_node(fn, std::move(st), out2));
+  n.in.push_back((int)fn->bld->fn.nodes.size() - 1);
+  n.second = true;
+  return add_node(fn, std::move(n), out);
+}
+
+int mx_fn_f8_quantize(mx_function* fn, mx_value xv, int block_rows, mx_value* codes, mx_value* scale) {
+  clear_error();
+  const char* op = "FusedF8Quantize";
+  MX_TRY(check_fn(fn, op));
+  if (!codes || !scale) return set_error(MX_ERR_INVALID, "%s: out is NULL", op);
+  int x;
+  MX_TRY(get_node(fn->bld, xv, op, &x));
+  const Shape xs = shape_of(fn, x);
+  if (!f32_or_bf16(xs.dtype))
+    return set_error(MX_ERR_NOT_IMPLEMENTED, "%s: x must be Float32 or BFloat16, got %s", op, dtype_name(xs.dtype));
+  if (block_rows != 1 && block_rows != MX_F8_BLOCK)
+    return set_error(MX_ERR_NOT_IMPLEMENTED, "%s: blockRows must be 1 or %d, got %d", op, MX_F8_BLOCK, block_rows);
+  if (xs.rank() < 1 || (block_rows != 1 && xs.rank() != 2))
+    return set_error(MX_ERR_INVALID, "%s: x must have rank %s, got %d", op, block_rows == 1 ? ">= 1" : "2 for 128 x 128 blocks", xs.rank());
+  Node n;
+  n.op = Op::kF8Quantize;
+  n.shape = xs;
+  n.shape.dtype = MX_DTYPE_F8E4M3FN;
+  n.in = {x};
+  n.rows = block_rows;
+  n.K = xs.dims.back();
+  n.M = 1;
+  for (int i = 0; i + 1 < xs.rank(); ++i) n.M *= xs.dims[i];
+  MX_TRY(f8_check_sizes(op, n.M, n.K, 0));
+  Shape ss = xs;
+  ss.dtype = MX_DTYPE_FLOAT32;
+  ss.dims.back() = f8_blocks(n.K);
+  if (block_rows != 1) ss.dims[0] = f8_blocks(n.M);
+  return add_two_outputs(fn, std::move(n), ss, codes, scale);
+}
+
+int mx_fn_f8_dense(mx_function* fn, mx_value xv, mx_value xsv, mx_value wv, mx_value wsv, mx_value biasv,
+                   const mx_f8_dense_config* config, mx_value* out) {
+  clear_error();
+  const char* op = "FusedF8Dense";
+  MX_TRY(check_fn(fn, op));
+  const mx_f8_dense_config cfg = config ? *config : mx_f8_dense_config{};
+  int x, xsc = -1, w, wsc, bias = -1;
+  MX_TRY(get_node(fn->bld, xv, op, &x));
+  if (xsv) MX_TRY(get_node(fn->bld, xsv, op, &xsc));
+  MX_TRY(get_node(fn->bld, wv, op, &w));
+  MX_TRY(get_node(fn->bld, wsv, op, &wsc));
+  if (biasv) MX_TRY(get_node(fn->bld, biasv, op, &bias));
+  const Shape xs = shape_of(fn, x), ws = shape_of(fn, w), wss = shape_of(fn, wsc);
+  Node n;
+  n.op = Op::kF8Dense;
+  if (xs.dtype == MX_DTYPE_F8E4M3FN) {
+    if (xsc < 0) return set_error(MX_ERR_INVALID, "%s: x in codes needs its scales", op);
+    MX_TRY(f8_check_rows(op, "x", xs, shape_of(fn, xsc), &n.M));
+  } else {
+    if (!f32_or_bf16(xs.dtype))
+      return set_error(MX_ERR_NOT_IMPLEMENTED, "%s: x must be F8E4M3FN, Float32 or BFloat16, got %s", op, dtype_name(xs.dtype));
+    if (xsc >= 0) return set_error(MX_ERR_INVALID, "%s: x in %s takes no scales", op, dtype_name(xs.dtype));
+    if (xs.rank() < 1) return set_error(MX_ERR_INVALID, "%s: x must have rank >= 1, got %d", op, xs.rank());
+    n.M = 1;
+    for (int i = 0; i + 1 < xs.rank(); ++i) n.M *= xs.dims[i];
+  }
+  if (cfg.weight_layout != MX_DENSE_LAYOUT_INPUT_OUTPUTS && cfg.weight_layout != MX_DENSE_LAYOUT_OUTPUTS_INPUT)
+    return set_error(MX_ERR_INVALID, "%s: unknown WeightLayout unknown", op);
+  n.oi = cfg.weight_layout == MX_DENSE_LAYOUT_OUTPUTS_INPUT;
+  n.K = xs.dims.back();
+  if (ws.dtype != MX_DTYPE_F8E4M3FN)
+    return set_error(MX_ERR_NOT_IMPLEMENTED, "%s: weights must be F8E4M3FN, got %s", op, dtype_name(ws.dtype));
+  if (ws.rank() != 2 || ws.dims[n.oi ? 1 : 0] != n.K)
+    return set_error(MX_ERR_INVALID, "%s: weights must be %s with K = %lld, got %s", op, n.oi ? "[N, K]" : "[K, N]", (long long)n.K,
+                     ws.str().c_str());
+  n.N = ws.dims[n.oi ? 0 : 1];
+  if (wss.dtype != MX_DTYPE_FLOAT32 || wss.rank() != 2 || wss.dims[0] != f8_blocks(ws.dims[0]) || wss.dims[1] != f8_blocks(ws.dims[1]))
+    return set_error(MX_ERR_INVALID, "%s: weight scales must be Float32 [%lld, %lld], got %s", op, (long long)f8_blocks(ws.dims[0]),
+                     (long long)f8_blocks(ws.dims[1]), wss.str().c_str());
+  if (bias >= 0) {
+    const Shape bs = shape_of(fn, bias);
+    if (bs.rank() != 1 || bs.dims[0] != n.N)
+      return set_error(MX_ERR_INVALID, "%s: bias must be [%lld], got %s", op, (long long)n.N, bs.str().c_str());
+    if (!f32_or_bf16(bs.dtype)) return set_error(MX_ERR_NOT_IMPLEMENTED, "%s: bias must be Float32 or BFloat16", op);
+  }
+  if (cfg.activation < MX_ACT_NONE || cfg.activation > MX_ACT_TANH)
+    return set_error(MX_ERR_INVALID, "%s: unknown activation %d", op, cfg.activation);
+  int odt = cfg.output_dtype;
+  if (odt == MX_DTYPE_INVALID) odt = xs.dtype == MX_DTYPE_F8E4M3FN ? MX_DTYPE_BFLOAT16 : xs.dtype;
+  if (!f32_or_bf16(odt))
+    return set_error(MX_ERR_NOT_IMPLEMENTED, "%s: OutputDType must be Float32 or BFloat16, got %s", op, dtype_name(odt));
+  MX_TRY(f8_check_sizes(op, n.M, n.K, n.N));
+  n.shape = xs;
+  n.shape.dtype = odt;
+  n.shape.dims.back() = n.N;
+  n.act = cfg.activation;
+  n.has_xs = xsc >= 0;
+  n.has_bias = bias >= 0;
+  n.in = {x, w, wsc};
+  if (n.has_xs) n.in.push_back(xsc);
+  if (n.has_bias) n.in.push_back(bias);
+  return add_node(fn, std::move(n), out);
+}
+
+int mx_fn_f8_weight_gradient(mx_function* fn, mx_value xv, mx_value xsv, mx_value dyv, int weight_layout,
+                             int output_dtype, mx_value* out) {
+  clear_error();
+  const char* op = "FusedF8WeightGradient";
+  MX_TRY(check_fn(fn, op));
+  int x, xsc, dy;
+  MX_TRY(get_node(fn->bld, xv, op, &x));
+  MX_TRY(get_node(fn->bld, xsv, op, &xsc));
+  MX_TRY(get_node(fn->bld, dyv, op, &dy));
+  const Shape xs = shape_of(fn, x), ds = shape_of(fn, dy);
+  Node n;
+  n.op = Op::kF8WGrad;
+  MX_TRY(f8_check_rows(op, "x", xs, shape_of(fn, xsc), &n.M));
+  if (!f32_or_bf16(ds.dtype))
+    return set_error(MX_ERR_NOT_IMPLEMENTED, "%s: dy must be Float32 or BFloat16, got %s", op, dtype_name(ds.dtype));
+  if (ds.rank() != xs.rank() || !std::equal(xs.dims.begin(), xs.dims.end() - 1, ds.dims.begin()))
+    return set_error(MX_ERR_INVALID, "%s: dy %s must have x's leading dimensions %s", op, ds.str().c_str(), xs.str().c_str());
+  if (weight_layout != MX_DENSE_LAYOUT_INPUT_OUTPUTS && weight_layout != MX_DENSE_LAYOUT_OUTPUTS_INPUT)
+    return set_error(MX_ERR_INVALID, "%s: unknown WeightLayout unknown", op);
+  const int odt = output_dtype == MX_DTYPE_INVALID ? MX_DTYPE_FLOAT32 : output_dtype;
+  if (!f32_or_bf16(odt))
+    return set_error(MX_ERR_NOT_IMPLEMENTED, "%s: OutputDType must be Float32 or BFloat16, got %s", op, dtype_name(odt));
+  n.K = xs.dims.back();
+  n.N = ds.dims.back();
+  n.oi = weight_layout == MX_DENSE_LAYOUT_OUTPUTS_INPUT;
+  MX_TRY(f8_check_sizes(op, n.M, n.K, n.N));
+  n.shape.dtype = odt;
+  n.shape.dims = n.oi ? std::vector<int64_t>{n.N, n.K} : std::vector<int64_t>{n.K, n.N};
+  n.in = {x, xsc, dy};
+  return add_node(fn, std::move(n), out);
+}
+
+int mx_fn_f8_activation_gradient(mx_function* fn, mx_value zv, mx_value zsv, mx_value upv, mx_value upsv, mx_value dyv,
+                                 int activation, mx_value* dz, mx_value* dup) {
+  clear_error();
+  const char* op = "FusedF8ActivationGradient";
+  MX_TRY(check_fn(fn, op));
+  if (!dz) return set_error(MX_ERR_INVALID, "%s: out is NULL", op);
+  if ((upv != 0) != (upsv != 0) || (upv != 0) != (dup != nullptr))
+    return set_error(MX_ERR_INVALID, "%s: up, its scales and the output dup come together", op);
+  int z, zsc, up = -1, upsc = -1, dy;
+  MX_TRY(get_node(fn->bld, zv, op, &z));
+  MX_TRY(get_node(fn->bld, zsv, op, &zsc));
+  if (upv) MX_TRY(get_node(fn->bld, upv, op, &up));
+  if (upsv) MX_TRY(get_node(fn->bld, upsv, op, &upsc));
+  MX_TRY(get_node(fn->bld, dyv, op, &dy));
+  const Shape zs = shape_of(fn, z), ds = shape_of(fn, dy);
+  Node n;
+  n.op = Op::kF8ActGrad;
+  MX_TRY(f8_check_rows(op, "z", zs, shape_of(fn, zsc), &n.M));
+  if (up >= 0) {
+    int64_t rows;
+    MX_TRY(f8_check_rows(op, "up", shape_of(fn, up), shape_of(fn, upsc), &rows));
+    if (shape_of(fn, up).dims != zs.dims)
+      return set_error(MX_ERR_INVALID, "%s: up %s must have z's shape %s", op, shape_of(fn, up).str().c_str(), zs.str().c_str());
+  }
+  if (!f32_or_bf16(ds.dtype))
+    return set_error(MX_ERR_NOT_IMPLEMENTED, "%s: dy must be Float32 or BFloat16, got %s", op, dtype_name(ds.dtype));
+  if (ds.dims != zs.dims)
+    return set_error(MX_ERR_INVALID, "%s: dy %s must have z's shape %s", op, ds.str().c_str(), zs.str().c_str());
+  if (activation < MX_ACT_NONE || activation > MX_ACT_TANH)
+    return set_error(MX_ERR_INVALID, "%s: unknown activation %d", op, activation);
+  n.N = zs.dims.back();
+  MX_TRY(f8_check_sizes(op, n.M, 0, n.N));
+  n.shape = ds;
+  n.act = activation;
+  n.in = {z, zsc, dy};
+  if (up < 0) return add_node(fn, std::move(n), dz);
+  n.in.push_back(up);
+  n.in.push_back(upsc);
+  return add_two_outputs(fn, std::move(n), ds, dz, dup);
+}
+
+// ---------------------------------------------------------------------------------------------
 // Elementwise and data movement.
 // ---------------------------------------------------------------------------------------------
 int mx_fn_unary(mx_function* fn, int optype, mx_value xv, mx_value* out) {
@@ -913,6 +1134,9 @@ int mx_fn_convert_dtype(mx_function* fn, mx_value xv, int dtype, mx_value* out) 
   MX_TRY(get_node(fn->bld, xv, "ConvertDType", &x));
   if (!dtype_known(dtype)) return set_error(MX_ERR_INVALID, "ConvertDType: unsupported dtype %d", dtype);
   const Shape xs = shape_of(fn, x);
+  if (dtype != xs.dtype && (dtype == MX_DTYPE_F8E4M3FN || xs.dtype == MX_DTYPE_F8E4M3FN))
+    return set_error(MX_ERR_NOT_IMPLEMENTED, "ConvertDType: conversion of %s to %s not implemented (FusedF8Quantize makes codes)",
+                     dtype_name(xs.dtype), dtype_name(dtype));
   if (dtype_is_packed(dtype))
     return set_error(MX_ERR_NOT_IMPLEMENTED, "ConvertDType: conversion to %s not implemented", dtype_name(dtype));
   Node n;
@@ -1302,8 +1526,10 @@ int mx_builder_compile(mx_builder* bld, mx_executable** out) {
   // Only nodes that feed the outputs are executed; find them.
   std::vector<bool> live(nn, false);
   for (int o : e->outputs) live[o] = true;
-  for (int i = nn - 1; i >= 0; --i)
+  for (int i = nn - 1; i >= 0; --i) {
+    if (e->nodes[i].second && live[e->nodes[i].in.back()]) live[i] = true;  // its second output is used
     if (live[i]) for (int j : e->nodes[i].in) live[j] = true;
+  }
   for (int p : e->params) live[p] = true;
   // Output claiming.
   std::vector<bool> claimed(nn, false);
@@ -1525,6 +1751,69 @@ static int run_node(mx_executable* e, int i, std::vector<void*>& ptr) {
       return ew_gelu(b, in(0), out, n.shape.dtype, count, n.flag & 1);
     case Op::kRmsNorm:
       return ew_rmsnorm(b, in(0), in(1), in(2), out, n.M, n.N);
+    case Op::kSecondOutput:
+      return MX_OK;  // written by the node that follows
+    case Op::kF8Quantize: {
+      F8QuantizeDesc d{};
+      d.x = in(0);
+      d.codes = (uint8_t*)out;
+      d.scale = (float*)in(1);
+      d.M = n.M;
+      d.K = n.K;
+      d.x_dt = ins(0).dtype;
+      d.rows = n.rows;
+      return f8_quantize_run(b, d);
+    }
+    case Op::kF8Dense: {
+      F8DenseDesc d{};
+      d.x = in(0);
+      d.w = (const uint8_t*)in(1);
+      d.w_scale = (const float*)in(2);
+      d.x_scale = n.has_xs ? (const float*)in(3) : nullptr;
+      const int kb = n.has_xs ? 4 : 3;
+      d.bias = n.has_bias ? in(kb) : nullptr;
+      d.b_dt = n.has_bias ? ins(kb).dtype : 0;
+      d.out = out;
+      d.M = n.M;
+      d.K = n.K;
+      d.N = n.N;
+      d.x_dt = ins(0).dtype;
+      d.out_dt = n.shape.dtype;
+      d.act = n.act;
+      d.oi = n.oi;
+      return f8_dense_run(b, d);
+    }
+    case Op::kF8WGrad: {
+      F8WGradDesc d{};
+      d.x = (const uint8_t*)in(0);
+      d.x_scale = (const float*)in(1);
+      d.dy = in(2);
+      d.out = out;
+      d.M = n.M;
+      d.K = n.K;
+      d.N = n.N;
+      d.dy_dt = ins(2).dtype;
+      d.out_dt = n.shape.dtype;
+      d.oi = n.oi;
+      return f8_wgrad_run(b, d);
+    }
+    case Op::kF8ActGrad: {
+      F8ActGradDesc d{};
+      d.z = (const uint8_t*)in(0);
+      d.z_scale = (const float*)in(1);
+      d.dy = in(2);
+      if (n.second) {
+        d.up = (const uint8_t*)in(3);
+        d.up_scale = (const float*)in(4);
+        d.dup = in(5);
+      }
+      d.dz = out;
+      d.M = n.M;
+      d.N = n.N;
+      d.dy_dt = ins(2).dtype;
+      d.act = n.act;
+      return f8_act_grad_run(b, d);
+    }
     case Op::kCopy:
       if (n.shape.nbytes())
         MX_CHECK_HIP(hipMemcpyAsync(out, in(0), n.shape.nbytes(), hipMemcpyDeviceToDevice, b->stream));
@@ -1542,7 +1831,9 @@ extern "C" int mx_exec_describe(const mx_executable* e, char* buf, size_t buflen
   std::string s;
   for (const Node& n : e->nodes) {
     if (n.flag & 0x100) continue;  // dead
-    if (n.op == Op::kParameter || n.op == Op::kConstant || n.op == Op::kReshape || n.op == Op::kBitcast) continue;
+    if (n.op == Op::kParameter || n.op == Op::kConstant || n.op == Op::kReshape || n.op == Op::kBitcast ||
+        n.op == Op::kSecondOutput)
+      continue;
     s += op_name(n.op);
     if (n.op == Op::kQDense && n.res_op) s += n.res_op == MX_OP_MUL ? "+Mul" : "+Add";
     if (n.op == Op::kQDense && n.pair) s += "+Pair";

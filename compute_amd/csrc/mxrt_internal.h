@@ -306,6 +306,54 @@ int dot_run(mx_backend* b, const DotDesc& d);
 bool dot_mfma_fits(const DotDesc& d);
 int dot_mfma_run(mx_backend* b, const DotDesc& d, const char* name);
 
+// Operators on 8-bit floating-point blocks (f8.cpp, f8_*.hip): e4m3 codes with a float32 scale per 128
+// values of a row, or per 128 x 128 block of a weight matrix.
+struct F8QuantizeDesc {
+  const void* x;   // [M, K] f32 / bf16
+  uint8_t* codes;  // [M, K]
+  float* scale;    // [M, KB], or [ceil(M / 128), KB] with rows == 128
+  int64_t M, K;
+  int x_dt, rows;
+};
+struct F8DenseDesc {
+  const void* x;         // [M, K] codes, or f32 / bf16
+  const float* x_scale;  // [M, KB] with codes
+  const uint8_t* w;      // [K, N], or [N, K] with oi
+  const float* w_scale;  // [KB, NB], or [NB, KB]
+  const void* bias;      // [N] or null
+  void* out;             // [M, N]
+  int64_t M, K, N;
+  int x_dt, b_dt, out_dt, act;
+  bool oi;
+};
+struct F8WGradDesc {
+  const uint8_t* x;      // [M, K]
+  const float* x_scale;  // [M, KB]
+  const void* dy;        // [M, N]
+  void* out;             // [K, N], or [N, K] with oi
+  int64_t M, K, N;
+  int dy_dt, out_dt;
+  bool oi;
+};
+struct F8ActGradDesc {
+  const uint8_t* z;       // [M, N]
+  const float* z_scale;   // [M, NB]
+  const uint8_t* up;      // or null
+  const float* up_scale;
+  const void* dy;         // [M, N]
+  void* dz;
+  void* dup;              // or null
+  int64_t M, N;
+  int dy_dt, act;
+};
+int f8_quantize_run(mx_backend* b, const F8QuantizeDesc& d);
+int f8_dense_run(mx_backend* b, const F8DenseDesc& d);    // makes float x into codes first
+int f8_product_run(mx_backend* b, const F8DenseDesc& d);  // x in codes
+const char* f8_product_name(const F8DenseDesc& d);
+int f8_wgrad_run(mx_backend* b, const F8WGradDesc& d);
+const char* f8_wgrad_name(const F8WGradDesc& d);
+int f8_act_grad_run(mx_backend* b, const F8ActGradDesc& d);
+
 // Elementwise / data-movement kernels (elementwise.hip).
 int ew_convert(mx_backend* b, const void* in, int in_dt, void* out, int out_dt, int64_t n);
 int ew_unary(mx_backend* b, int optype, const void* in, void* out, int dt, int64_t n);

@@ -50,6 +50,7 @@ const char* dtype_name(int dt) {
     case MX_DTYPE_FLOAT32: return "Float32";
     case MX_DTYPE_FLOAT64: return "Float64";
     case MX_DTYPE_BFLOAT16: return "BFloat16";
+    case MX_DTYPE_F8E4M3FN: return "F8E4M3FN";
     case MX_DTYPE_INT4: return "Int4";
     case MX_DTYPE_UINT4: return "Uint4";
     default: return "InvalidDType";
@@ -60,7 +61,8 @@ int dtype_bits(int dt) {
   switch (dt) {
     case MX_DTYPE_BOOL:
     case MX_DTYPE_INT8:
-    case MX_DTYPE_UINT8: return 8;
+    case MX_DTYPE_UINT8:
+    case MX_DTYPE_F8E4M3FN: return 8;
     case MX_DTYPE_INT16:
     case MX_DTYPE_UINT16:
     case MX_DTYPE_FLOAT16:
@@ -475,7 +477,7 @@ int mx_backend_supports_dtype(const mx_backend* b, int dtype, int* out) {
     case MX_DTYPE_INT8: case MX_DTYPE_INT16: case MX_DTYPE_INT32: case MX_DTYPE_INT64:
     case MX_DTYPE_UINT8: case MX_DTYPE_UINT16: case MX_DTYPE_UINT32: case MX_DTYPE_UINT64:
     case MX_DTYPE_FLOAT16: case MX_DTYPE_FLOAT32: case MX_DTYPE_FLOAT64: case MX_DTYPE_BFLOAT16:
-    case MX_DTYPE_INT4: case MX_DTYPE_UINT4: case MX_DTYPE_BOOL:
+    case MX_DTYPE_INT4: case MX_DTYPE_UINT4: case MX_DTYPE_BOOL: case MX_DTYPE_F8E4M3FN:
       *out = 1;
       break;
     default:

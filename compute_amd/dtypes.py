@@ -29,6 +29,7 @@ class DType(enum.IntEnum):
     Float32 = 11
     Float64 = 12
     BFloat16 = 13
+    F8E4M3FN = 17
     Int4 = 21
     Uint4 = 22
 
@@ -67,7 +68,7 @@ _BITS = {
     DType.InvalidDType: 0, DType.Bool: 8, DType.Int8: 8, DType.Int16: 16, DType.Int32: 32,
     DType.Int64: 64, DType.Uint8: 8, DType.Uint16: 16, DType.Uint32: 32, DType.Uint64: 64,
     DType.Float16: 16, DType.Float32: 32, DType.Float64: 64, DType.BFloat16: 16, DType.Int4: 4,
-    DType.Uint4: 4,
+    DType.Uint4: 4, DType.F8E4M3FN: 8,
 }
 
 _NP = {
@@ -76,7 +77,7 @@ _NP = {
     DType.Uint16: np.dtype(np.uint16), DType.Uint32: np.dtype(np.uint32), DType.Uint64: np.dtype(np.uint64),
     DType.Float16: np.dtype(np.float16), DType.Float32: np.dtype(np.float32),
     DType.Float64: np.dtype(np.float64), DType.BFloat16: np.dtype(np.uint16),
-    DType.Int4: np.dtype(np.uint8), DType.Uint4: np.dtype(np.uint8),
+    DType.Int4: np.dtype(np.uint8), DType.Uint4: np.dtype(np.uint8), DType.F8E4M3FN: np.dtype(np.uint8),
 }
 
 # Re-exported names, as the reference's `dtypes.X`.
@@ -85,6 +86,7 @@ InvalidDType, Bool, Int8, Int16, Int32, Int64 = (DType.InvalidDType, DType.Bool,
 Uint8, Uint16, Uint32, Uint64 = DType.Uint8, DType.Uint16, DType.Uint32, DType.Uint64
 Float16, Float32, Float64, BFloat16, Int4, Uint4 = (DType.Float16, DType.Float32, DType.Float64, DType.BFloat16,
                                                     DType.Int4, DType.Uint4)
+F8E4M3FN = DType.F8E4M3FN
 
 
 @dataclass(frozen=True)

@@ -60,6 +60,10 @@ enum {
   MX_DTYPE_FLOAT32 = 11,
   MX_DTYPE_FLOAT64 = 12,
   MX_DTYPE_BFLOAT16 = 13,
+  MX_DTYPE_F8E4M3FN = 17, /* OCP 8-bit float: 4 exponent bits (bias 7), 3 of mantissa, largest 448, no
+                             infinities, NaN 0x7f / 0xff.  Taken by the MX_OP_F8_* operators and by
+                             the ops that only move data (Parameter, Constant, Reshape, Bitcast,
+                             Transpose, Slice, BroadcastInDim, Identity) */
   MX_DTYPE_INT4 = 21,  /* packed, 2 per byte, low nibble first (dtypes/dtypes.go:175-239) */
   MX_DTYPE_UINT4 = 22
 };
@@ -121,7 +125,13 @@ enum {
   MX_OP_FUSED_GELU = 118,
   MX_OP_FUSED_DENSE = 119,
   MX_OP_FUSED_QUANTIZED_DENSE = 123,
-  MX_OP_QUANTIZED_EMBEDDING_LOOKUP = 124
+  MX_OP_QUANTIZED_EMBEDDING_LOOKUP = 124,
+  /* Operators on 8-bit floating-point blocks: no counterpart in the reference's enum, so numbered
+   * apart from it. */
+  MX_OP_F8_QUANTIZE = 1000,
+  MX_OP_F8_DENSE = 1001,
+  MX_OP_F8_WEIGHT_GRADIENT = 1002,
+  MX_OP_F8_ACTIVATION_GRADIENT = 1003
 };
 
 #define MX_MAX_RANK 8
@@ -327,6 +337,54 @@ int mx_fn_fused_dense(mx_function* fn, mx_value x, mx_value weight, mx_value bia
 /* FusedOps.FusedGelu (fused_ops.go:329). */
 int mx_fn_fused_gelu(mx_function* fn, mx_value x, int exact, mx_value* out);
 
+/* ---------------------------------------------------------------------------------------------
+ * Operators on 8-bit floating-point blocks (no counterpart in the reference; the conventions are
+ * those of FusedQuantizedDense and FusedDense).
+ *
+ * The format: e4m3 codes (MX_DTYPE_F8E4M3FN) and float32 scales; a value is code * scale.  A row has
+ * one scale for every MX_F8_BLOCK consecutive codes (the last block of a row may be shorter): codes
+ * [batch..., K], scale [batch..., ceil(K/128)].  A weight matrix has one scale for every 128 x 128
+ * block: codes [R, C], scale [ceil(R/128), ceil(C/128)].
+ * ------------------------------------------------------------------------------------------- */
+#define MX_F8_BLOCK 128
+
+/* Codes and scales of x (float32 or bfloat16).  block_rows 1: x [batch..., K], one scale per row
+ * block; block_rows 128: x [R, C], one per 128 x 128 block.  With a the largest finite magnitude of a
+ * block, its scale is the smallest power of two s with a <= 448 s (at least 2^-126; 1 where a is 0)
+ * and a code is x / s, exact, rounded to nearest even; infinities and NaN become NaN. */
+int mx_fn_f8_quantize(mx_function* fn, mx_value x, int block_rows, mx_value* codes, mx_value* scale);
+
+typedef struct mx_f8_dense_config {
+  int32_t activation;    /* MX_ACT_*                                                          */
+  int32_t weight_layout; /* MX_DENSE_LAYOUT_*: weight [in, out] or [out, in]                   */
+  int32_t output_dtype;  /* float32 or bfloat16; MX_DTYPE_INVALID: x's dtype, bfloat16 for codes */
+} mx_f8_dense_config;
+/* y = act(x W + bias) over blocks.  x: codes [batch..., K] with x_scale, or float32 / bfloat16 values
+ * with x_scale 0, which the operator itself first makes into codes and scales as mx_fn_f8_quantize
+ * does.  weight: codes [K, N] or [N, K] (weight_layout) with 128 x 128-block scales; bias: [N]
+ * float32 or bfloat16, or 0.  Each block's sum of products of codes is formed by itself and enters
+ * the float32 sum as (x_scale * w_scale) * sum; a product of two scales has to be finite.  The
+ * weight of a forward pass, read in the other layout, gives the input gradient dy W^T.  config NULL:
+ * the zero config. */
+int mx_fn_f8_dense(mx_function* fn, mx_value x, mx_value x_scale, mx_value weight, mx_value weight_scale,
+                   mx_value bias, const mx_f8_dense_config* config, mx_value* out);
+
+/* The weight gradient of a dense layer from its input kept in 8 bits: x^T dy, summed in float32 over
+ * all leading dimensions.  x: codes [batch..., K] with x_scale; dy [batch..., N] float32 or bfloat16;
+ * output [K, N] or [N, K] (weight_layout), float32 or bfloat16 (MX_DTYPE_INVALID: float32).  A value
+ * of x enters as code * scale in bfloat16, which is exact for scales that are powers of two, as
+ * mx_fn_f8_quantize makes them; float32 dy enters with all its bits (down to magnitudes of 2^-110). */
+int mx_fn_f8_weight_gradient(mx_function* fn, mx_value x, mx_value x_scale, mx_value dy, int weight_layout,
+                             int output_dtype, mx_value* out);
+
+/* The gradient of an activation from its input kept in 8 bits: dz = dy * act'(z), and with up (codes
+ * and scales of z's shape; 0: none) that of the gated product act(z) * up: dz = dy * up * act'(z),
+ * dup = dy * act(z).  z: codes [batch..., N] with z_scale; dy: z's shape, float32 or bfloat16; dz and
+ * dup have dy's shape and dtype.  At a corner of the activation the slope is the left one (ReLU: 0 at
+ * 0; HardSwish: 0 up to -3) or, for HardSwish at 3, 1.  dup may be NULL exactly where up is 0. */
+int mx_fn_f8_activation_gradient(mx_function* fn, mx_value z, mx_value z_scale, mx_value up, mx_value up_scale,
+                                 mx_value dy, int activation, mx_value* dz, mx_value* dup);
+
 /* Elementwise ops: optype is one of MX_OP_ABS/NEG/EXP/ERF/LOGISTIC/RSQRT/SQRT/TANH/IDENTITY
  * (unary; standard_ops.go:134,418,421,524,577,590,741,823,830) or MX_OP_ADD/SUB/MUL/DIV/MAX/MIN
  * (binary; standard_ops.go:138,337,580,583,587,827). */
@@ -438,6 +496,60 @@ typedef struct mx_qembed_args {
   int32_t index_dtype, ggml_type;
 } mx_qembed_args;
 int mx_quantized_embedding_lookup(mx_backend* b, const mx_qembed_args* args);
+
+/* ---------------------------------------------------------------------------------------------
+ * The operators on 8-bit floating-point blocks on device pointers (the Executable launches the same
+ * kernels), on the backend's stream, asynchronous.  Arrays are contiguous; outputs must not overlap
+ * inputs, except that dz may be dy itself.  Rows and columns are below 2^30.  mx_f8_dense with float x
+ * takes the codes' memory from the backend's pool; the other calls allocate nothing.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct mx_f8_quantize_args {
+  const void* x;      /* [M, K], x_dtype                                                      */
+  void* codes;        /* [M, K]                                                               */
+  float* scale;       /* [M, ceil(K/128)], or [ceil(M/128), ceil(K/128)] with block_rows 128   */
+  int64_t M, K;
+  int32_t x_dtype, block_rows;
+} mx_f8_quantize_args;
+int mx_f8_quantize(mx_backend* b, const mx_f8_quantize_args* args);
+
+typedef struct mx_f8_dense_args {
+  const void* x;         /* [M, K], x_dtype: MX_DTYPE_F8E4M3FN, float32 or bfloat16            */
+  const float* x_scale;  /* [M, ceil(K/128)] with codes; NULL with float x                     */
+  const void* w;         /* codes [K, N] or [N, K]                                             */
+  const float* w_scale;  /* [ceil(K/128), ceil(N/128)] or [ceil(N/128), ceil(K/128)]           */
+  const void* bias;      /* [N], bias_dtype, or NULL                                           */
+  void* out;             /* [M, N], out_dtype                                                  */
+  int64_t M, K, N;
+  int32_t x_dtype, bias_dtype, out_dtype, weight_layout, activation;
+} mx_f8_dense_args;
+int mx_f8_dense(mx_backend* b, const mx_f8_dense_args* args);
+/* Name of the kernel that mx_f8_dense would launch for the product of these arguments. */
+int mx_f8_dense_plan(mx_backend* b, const mx_f8_dense_args* args, char* buf, size_t buflen);
+
+typedef struct mx_f8_weight_grad_args {
+  const void* x;         /* codes [M, K]                                                       */
+  const float* x_scale;  /* [M, ceil(K/128)]                                                   */
+  const void* dy;        /* [M, N], dy_dtype                                                   */
+  void* out;             /* [K, N] or [N, K], out_dtype                                        */
+  int64_t M, K, N;
+  int32_t dy_dtype, out_dtype, weight_layout;
+} mx_f8_weight_grad_args;
+int mx_f8_weight_gradient(mx_backend* b, const mx_f8_weight_grad_args* args);
+/* Name of the kernel that mx_f8_weight_gradient would launch for these arguments. */
+int mx_f8_weight_gradient_plan(mx_backend* b, const mx_f8_weight_grad_args* args, char* buf, size_t buflen);
+
+typedef struct mx_f8_act_grad_args {
+  const void* z;          /* codes [M, N]                                                      */
+  const float* z_scale;   /* [M, ceil(N/128)]                                                  */
+  const void* up;         /* codes [M, N], or NULL                                             */
+  const float* up_scale;  /* [M, ceil(N/128)], or NULL                                         */
+  const void* dy;         /* [M, N], dy_dtype                                                  */
+  void* dz;               /* [M, N], dy_dtype                                                  */
+  void* dup;              /* [M, N], dy_dtype, or NULL                                         */
+  int64_t M, N;
+  int32_t dy_dtype, activation;
+} mx_f8_act_grad_args;
+int mx_f8_activation_gradient(mx_backend* b, const mx_f8_act_grad_args* args);
 
 #ifdef __cplusplus
 }
