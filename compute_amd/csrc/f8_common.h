@@ -47,6 +47,50 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
+// 16 bytes from p, of which the first n are there (the rest 0).  p may be any byte.
+__device__ __forceinline__ u32x4 load16(const uint8_t* p, int64_t n) {
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (n >= 16) {
+    __builtin_memcpy(&v, p, 16);
+  } else {
+    for (int i = 0; i < n; ++i) v[i / 4] |= (uint32_t)p[i] << (8 * (i % 4));
+  }
+  return v;
+}
+
+// Workgroup barrier ordering LDS only: global loads in flight stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// LDS byte address of a shared-memory pointer.
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+// Transposing LDS reads: every 16 lanes read a block of 16 columns, lane l's eight bytes lying at its
+// own address, and lane i gets column i.  16-bit values: four rows, of which lane l holds row l / 4,
+// columns 4 (l % 4) ..; codes: eight rows, lane l row l / 2, columns 8 (l % 2) ...
+__device__ __forceinline__ u32x2 read_tr16(uint32_t addr) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)addr));
+}
+__device__ __forceinline__ u32x2 read_tr8(uint32_t addr) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)addr));
+}
+
+// Workgroup b of n to a work item such that each XCD (the hardware deals workgroups to the eight in
+// turn) takes a contiguous run of items.
+__device__ __forceinline__ int xcd_order(int b, int n) {
+  constexpr int kXcds = 8;
+  const int x = b % kXcds, q = n / kXcds, r = n % kXcds;
+  return x * q + (x < r ? x : r) + b / kXcds;
+}
+
 // The magnitude bits of a finite value, 0 of an infinity or NaN: they compare as integers.
 __device__ __forceinline__ uint32_t finite_bits(float v) {
   const uint32_t u = __float_as_uint(v) & 0x7fffffffu;

@@ -56,17 +56,6 @@ __device__ __forceinline__ f32x4 block_sum(const i32x8& a, const i32x8& b) {
   }
 }
 
-// 16 bytes from p, of which the first n are in the row (the rest 0).  Rows may start at any byte.
-__device__ __forceinline__ u32x4 load16(const uint8_t* p, int n) {
-  u32x4 v = {0u, 0u, 0u, 0u};
-  if (n >= 16) {
-    __builtin_memcpy(&v, p, 16);
-  } else {
-    for (int i = 0; i < n; ++i) v[i / 4] |= (uint32_t)p[i] << (8 * (i % 4));
-  }
-  return v;
-}
-
 // Any sizes, alignment and layout: 64 x 64 tiles, both operands staged in LDS as rows of 128 codes.
 constexpr int kAnyTile = 64, kAnyThreads = 256, kAnyPitch = kBlock + 16;
 
