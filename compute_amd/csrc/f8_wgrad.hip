@@ -46,26 +46,56 @@ __device__ __forceinline__ void parts_of(float v, uint16_t (&p)[3]) {
   p[2] = (uint16_t)(__float_as_uint(r2) >> 16);
 }
 
-// A workgroup of four waves computes 32 T (k) x 32 T (n), a wave 16 T x 16 T of it; tokens in steps of S.
+// A workgroup computes W (k) x W (n) in WK x WN waves of 16 TK x 16 TN; tokens in steps of S.
+template <int WK_, int WN_, int TK_, int TN_, int S_, int OCC>
+struct Tile {
+  static constexpr int WK = WK_, WN = WN_, TK = TK_, TN = TN_, S = S_, W = 16 * TK * WK, kThreads = 64 * WK * WN, kOccupancy = OCC;
+  static_assert(W == 16 * TN * WN, "square tiles");
+};
 //
-// Per step the codes and dy travel through registers, requested one step ahead: 16 codes a chunk, scaled
-// to bf16 (32 bytes of LDS), and 8 values of dy.  LDS keeps both as they lie in memory, [token][column],
-// in two buffers; the operands, eight consecutive tokens of a column per lane, come out through the
-// transposing read, four tokens at a time.  A row's 32-byte pieces are XOR-ed with (token & 3) | (token
-// >> 3 & 1) << 2, so that the 32 lanes of a half-wave, which read 8 rows of one piece, touch every bank
-// once.
+// Staging.  The codes and dy of a step travel through registers, requested a step ahead: 16 codes a chunk,
+// scaled to bf16 (32 bytes of LDS), and 8 values of dy.  LDS keeps both as they lie in memory,
+// [token][column], in two buffers; the operands, eight consecutive tokens of a column per lane, come out
+// through the transposing read, four tokens at a time.  A row's 32-byte pieces are XOR-ed with (token & 3)
+// | (token >> 3 & 1) << 2, so that the 32 lanes of a half-wave, which read 8 rows of one piece, touch
+// every bank once.
+//
+// Schedule.  A step is G groups of TK MFMAs, one operand of dy against the wave's TK operands of x.  An
+// operand of dy is read kRing - 1 groups ahead of its use and the x operands of the next 32 tokens
+// during the present ones.  The step's barrier stands before its last kRing - 1 groups, whose operands
+// are then in registers: under them travel the first operands of the next step.  A chunk of the next step
+// is staged, and that of the step after requested into its registers, in the groups before the barrier.
 //
 // Columns past K or N hold whatever lies there: they meet only results that are not stored.  Tokens past
-// M are zeros in both operands.  WHOLE: rows are whole chunks; otherwise a chunk may start anywhere and
-// run into the next row, and only the array's own end is looked at.
-template <int T, int S, bool F32, bool OI, bool WHOLE>
-__global__ __launch_bounds__(256, 1) void f8_wgrad_kernel(WGradArgs a) {
-  constexpr int P = F32 ? 3 : 1, W = 32 * T;           // parts of dy, columns of a tile
+// M are zeros in both operands (a step past the last is staged like any other and not used).  WHOLE: rows
+// are whole chunks below 2^24 columns, read through buffer resources that end with the array, so that
+// what lies past it reads as zero; otherwise a chunk may start anywhere and run into the next row, and the
+// tokens and the array's end are looked at.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const void* p, int64_t bytes) {
+  const int64_t n = bytes < 0 ? 0 : bytes < 0xffffffffll ? bytes : 0xffffffffll;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)(uint32_t)n, 0x00027000);
+}
+
+template <class Tile, bool F32, bool OI, bool WHOLE>
+__global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_kernel(WGradArgs a) {
+  constexpr int TK = Tile::TK, TN = Tile::TN, S = Tile::S, kThreads = Tile::kThreads;
+  constexpr int P = F32 ? 3 : 1, W = Tile::W;          // parts of dy, columns of a tile
   constexpr int kRow = 2 * W;                          // bytes of a row in LDS
   constexpr int kBuf = S * kRow;                       // one operand (part) of a step
-  constexpr int CX = S * W / 16 / 256;                 // chunks of x a thread stages
-  constexpr int CD = S * W / 8 / 256;                  // chunks of dy
-  static_assert(CX * 16 * 256 == S * W && CD * 8 * 256 == S * W, "whole chunks");
+  constexpr int kStep = (1 + P) * kBuf;                // LDS of a step
+  constexpr int CX = S * W / 16 / kThreads;            // chunks of x a thread stages
+  constexpr int CD = S * W / 8 / kThreads;             // chunks of dy
+  constexpr int RX = kThreads / (W / 16), RD = kThreads / (W / 8);  // rows between a thread's chunks
+  constexpr int kHalves = S / 32, G = kHalves * P * TN;
+  constexpr int kRing = 4, kLast = kRing - 1;          // groups after the barrier
+  constexpr int kPieces = CX + CD;
+  constexpr int kStageGroups = G - kLast < kPieces ? G - kLast : kPieces, kStageFrom = G - kLast - kStageGroups;
+  constexpr int kPerGroup = (kPieces + kStageGroups - 1) / kStageGroups;
+  constexpr int H = F32 ? 2 : 1, E = F32 ? 4 : 2;      // loads of a dy chunk, bytes of a value
+  static_assert(CX * 16 * kThreads == S * W && CD * 8 * kThreads == S * W, "whole chunks");
+  static_assert(G % kRing == 0, "the ring's slots are the same in every step");
+  static_assert((kStep & (kStep - 1)) == 0, "the buffers alternate by an XOR");
+  static_assert((TK & (TK - 1)) == 0 && (TN & (TN - 1)) == 0, "a wave's pieces start on a multiple of their number: an XOR picks one");
   extern __shared__ __align__(1024) uint8_t lds[];     // [2][1 + P][S][W] bf16
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, i = lane % 16, g = lane / 16;
   const int tiles_k = (a.K + W - 1) / W;
@@ -79,64 +109,69 @@ __global__ __launch_bounds__(256, 1) void f8_wgrad_kernel(WGradArgs a) {
   }
   const int k0 = kt * W, n0 = nt * W;
   const int64_t x_total = (int64_t)a.M * a.K, dy_total = (int64_t)a.M * a.N;
+  const int xrow = tid / (W / 16), xk = k0 + 16 * (tid % (W / 16));  // the thread's first chunk of a step
+  const int drow = tid / (W / 8), dn = n0 + 8 * (tid % (W / 8));
+  const int kb = min(xk / kBlock, a.KB - 1);
 
-  u32x4 xr[CX], dr[CD][F32 ? 2 : 1];
+  u32x4 xr[CX], dr[CD][H];
   float sr[CX];
-  auto request = [&](int m0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < CX; ++j) {
-      const int c = tid + 256 * j, m = m0 + c / (W / 16), k = k0 + 16 * (c % (W / 16));
-      const int mc = min(m, a.M - 1);
-      const int64_t row = (int64_t)mc * a.K;
+  // Byte offsets of the first chunk within a step (WHOLE: below 64 rows of 2^26 bytes).
+  const uint32_t x_off = (uint32_t)xrow * (uint32_t)a.K + (uint32_t)min(xk, a.K - 16);
+  const uint32_t s_off = 4 * ((uint32_t)xrow * (uint32_t)a.KB + (uint32_t)kb);
+  const uint32_t d_off = E * ((uint32_t)drow * (uint32_t)a.N + (uint32_t)min(dn, a.N - 8));
+  auto request = [&](int m0, int piece) __attribute__((always_inline)) {
+    if (piece < CX) {
+      const int j = piece;
       if constexpr (WHOLE) {
-        xr[j] = *(const u32x4*)(a.x + row + min(k, a.K - 16));
+        const int64_t m = m0 + j * RX;
+        xr[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(resource(a.x + m * a.K, x_total - m * a.K), x_off, 0, 0));
+        sr[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                              resource(a.x_scale + m * a.KB, ((int64_t)a.M - m) * a.KB * 4), s_off, 0, 0));
       } else {
-        const int64_t at = row + min(k, a.K - 1);
+        const int64_t row = min(m0 + xrow + j * RX, a.M - 1), at = row * a.K + min(xk, a.K - 1);
         xr[j] = load16(a.x + at, x_total - at);
+        sr[j] = a.x_scale[row * a.KB + kb];
       }
-      sr[j] = a.x_scale[(int64_t)mc * a.KB + min(k / kBlock, a.KB - 1)];
-      if (m >= a.M) xr[j] = u32x4{0u, 0u, 0u, 0u};
-    }
+    } else if (piece < kPieces) {
+      const int j = piece - CX;
 #pragma unroll
-    for (int j = 0; j < CD; ++j) {
-      const int c = tid + 256 * j, m = m0 + c / (W / 8), n = n0 + 8 * (c % (W / 8));
-      const int64_t row = (int64_t)min(m, a.M - 1) * a.N;
-      constexpr int E = F32 ? 4 : 2;
-      const uint8_t* p = (const uint8_t*)a.dy;
-#pragma unroll
-      for (int h = 0; h < (F32 ? 2 : 1); ++h) {
+      for (int h = 0; h < H; ++h) {
         if constexpr (WHOLE) {
-          dr[j][h] = *(const u32x4*)(p + E * (row + min(n, a.N - 8)) + 16 * h);
+          const int64_t at = (int64_t)(m0 + j * RD) * a.N;
+          dr[j][h] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                   resource((const uint8_t*)a.dy + at * E, (dy_total - at) * E), d_off, 16 * h, 0));
         } else {
-          const int64_t at = row + min(n, a.N - 1) + 4 * h;
-          dr[j][h] = load16(p + E * at, E * (dy_total - at));
+          const int64_t at = (int64_t)min(m0 + drow + j * RD, a.M - 1) * a.N + min(dn, a.N - 1) + 4 * h;
+          dr[j][h] = load16((const uint8_t*)a.dy + E * at, E * (dy_total - at));
         }
-        if (m >= a.M) dr[j][h] = u32x4{0u, 0u, 0u, 0u};
       }
     }
   };
+  // Piece of the step from m0 into LDS at `step`.
   auto swizzled = [](int m, int piece) { return m * kRow + 32 * (piece ^ ((m & 3) | (m >> 3 & 1) << 2)); };
-  auto stage = [&](int buf) __attribute__((always_inline)) {
-    uint8_t* xb = lds + buf * (1 + P) * kBuf;
-#pragma unroll
-    for (int j = 0; j < CX; ++j) {
-      const int c = tid + 256 * j;
+  auto stage = [&](int m0, uint32_t step, int piece) __attribute__((always_inline)) {
+    uint8_t* xb = lds + step;
+    if (piece < CX) {
+      const int j = piece;
+      if (!WHOLE && m0 + xrow + j * RX >= a.M) xr[j] = u32x4{0u, 0u, 0u, 0u};
       u32x4 o[2];
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const f32x4 v = decode4(xr[j][w]);
-        const f32x2 lo = {v[0] * sr[j], v[1] * sr[j]}, hi = {v[2] * sr[j], v[3] * sr[j]};
+        const float s = sr[j];
+        const f32x2 lo = {v[0] * s, v[1] * s}, hi = {v[2] * s, v[3] * s};
         o[w / 2][2 * (w % 2)] = __builtin_bit_cast(uint32_t, __builtin_convertvector(lo, bf16x2));
         o[w / 2][2 * (w % 2) + 1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(hi, bf16x2));
       }
-      uint8_t* q = xb + swizzled(c / (W / 16), c % (W / 16));
+      uint8_t* q = xb + swizzled(xrow + j * RX, tid % (W / 16));
       *(u32x4*)q = o[0];
       *(u32x4*)(q + 16) = o[1];
-    }
+    } else if (piece < kPieces) {
+      const int j = piece - CX, c = tid % (W / 8);
 #pragma unroll
-    for (int j = 0; j < CD; ++j) {
-      const int c = tid + 256 * j, piece = c % (W / 8);
-      uint8_t* q = xb + kBuf + swizzled(c / (W / 8), piece / 2) + 16 * (piece % 2);
+      for (int h = 0; h < H; ++h)
+        if (!WHOLE && m0 + drow + j * RD >= a.M) dr[j][h] = u32x4{0u, 0u, 0u, 0u};
+      uint8_t* q = xb + kBuf + swizzled(drow + j * RD, c / 2) + 16 * (c % 2);
       if constexpr (F32) {
         uint16_t p[8][3];
 #pragma unroll
@@ -155,66 +190,99 @@ __global__ __launch_bounds__(256, 1) void f8_wgrad_kernel(WGradArgs a) {
   };
 
   // Operand reads: token 8 g + 4 h + i / 4 of a half step, columns 16 t + 4 (i % 4) ..
-  const int wk = wave / 2, wn = wave % 2;
+  const int wk = wave / Tile::WN, wn = wave % Tile::WN;
   const uint32_t base = lds_addr(lds);
-  auto read_base = [&](int w) { return base + (uint32_t)swizzled(8 * g + i / 4, w * T) + 8 * (i % 4); };
-  const uint32_t xa = read_base(wk), da = read_base(wn) + kBuf;
+  auto read_base = [&](int piece) { return base + (uint32_t)swizzled(8 * g + i / 4, piece) + 8 * (i % 4); };
+  const uint32_t xa = read_base(wk * TK), da = read_base(wn * TN) + kBuf;
   auto operand = [&](uint32_t at, int t, int off) __attribute__((always_inline)) {
     const uint32_t p = (at ^ (uint32_t)(32 * t)) + (uint32_t)off;
     const u32x2 lo = read_tr16(p), hi = read_tr16(p + 4 * kRow);
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
-  static_assert(T == 4 || T == 8, "a wave's pieces start on a multiple of its own T, so an XOR with t < T picks one");
-
-  f32x4 acc[T][T] = {};
-  auto multiply = [&](int buf) __attribute__((always_inline)) {
-#pragma unroll
-    for (int h = 0; h < S / 32; ++h) {
-      const int off = buf * (1 + P) * kBuf + h * 32 * kRow;
-      u32x4 xo[T], dv;
-#pragma unroll
-      for (int t = 0; t < T; ++t) xo[t] = operand(xa, t, off);
-#pragma unroll
-      for (int p = P - 1; p >= 0; --p)
-#pragma unroll
-        for (int n = 0; n < T; ++n) {
-          dv = operand(da, n, off + p * kBuf);
-#pragma unroll
-          for (int t = 0; t < T; ++t) {
-            if constexpr (OI)
-              acc[t][n] = mfma_bf16(dv, xo[t], acc[t][n]);
-            else
-              acc[t][n] = mfma_bf16(xo[t], dv, acc[t][n]);
-          }
-        }
-    }
+  u32x4 xo[2][TK], dv[kRing];
+  auto read_x = [&](int set, int t, uint32_t step, int half) __attribute__((always_inline)) {
+    xo[set][t] = operand(xa + step, t, half * 32 * kRow);
+  };
+  auto read_dy = [&](int q, uint32_t step) __attribute__((always_inline)) {  // of group q of a step
+    dv[q % kRing] = operand(da + step, q % TN, (q / TN % P) * kBuf + q / (TN * P) * 32 * kRow);
   };
 
-  const int steps = (a.M + S - 1) / S;
-  if (steps > 0) {
-    request(0);
-    stage(0);
-    lds_barrier();
-    for (int s = 0; s < steps; s += 2) {
+  f32x4 acc[TK][TN] = {};
+  if (a.M > 0) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if (s + b < steps) {
-          const bool more = s + b + 1 < steps;
-          if (more) request((s + b + 1) * S);
-          multiply(b);
-          if (more) stage(1 - b);
-          lds_barrier();
+    for (int p = 0; p < kPieces; ++p) request(0, p);
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      stage(0, 0, p);
+      request(S, p);
+    }
+    lds_barrier();
+#pragma unroll
+    for (int t = 0; t < TK; ++t) read_x(0, t, 0, 0);
+#pragma unroll
+    for (int q = 0; q < kLast; ++q) read_dy(q, 0);
+    uint32_t cur = 0;
+    for (int m0 = 0; m0 < a.M; m0 += S) {
+      const uint32_t next = cur ^ kStep;
+#pragma unroll
+      for (int q = 0; q < G; ++q) {
+        constexpr int kHalf = TN * P;
+        const int half = q / kHalf, set = half % 2;
+        if (q == G - kLast) lds_barrier();
+        // Operands of later groups.
+        if (q + kLast < G)
+          read_dy(q + kLast, cur);
+        else
+          read_dy(q + kLast - G, next);
+        if (half + 1 < kHalves && q % kHalf < TK) read_x(1 - set, q % kHalf, cur, half + 1);
+        if (q >= G - kLast) {
+          constexpr int per = (TK + kLast - 1) / kLast;
+#pragma unroll
+          for (int e = 0; e < per; ++e) {
+            const int t = (q - (G - kLast)) * per + e;
+            if (t < TK) read_x(1 - set, t, next, 0);
+          }
+        }
+        if (q >= kStageFrom && q < G - kLast) {
+#pragma unroll
+          for (int e = 0; e < kPerGroup; ++e) {
+            const int p = (q - kStageFrom) * kPerGroup + e;
+            stage(m0 + S, next, p);
+            request(m0 + 2 * S, p);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < TK; ++t) {
+          if constexpr (OI)
+            acc[t][q % TN] = mfma_bf16(dv[q % kRing], xo[set][t], acc[t][q % TN]);
+          else
+            acc[t][q % TN] = mfma_bf16(xo[set][t], dv[q % kRing], acc[t][q % TN]);
+        }
+        if constexpr (WHOLE) {
+#pragma unroll
+          for (int t = 0; t < TK; ++t) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+            __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);  // VALU
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);  // LDS write
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
+      if constexpr (kHalves == 1) {
+#pragma unroll
+        for (int t = 0; t < TK; ++t) xo[0][t] = xo[1][t];
+      }
+      cur = next;
     }
   }
 
   // Result (t, n): rows 4 g + r and column i of its 16 x 16; OI: rows are columns of dy.
 #pragma unroll
-  for (int t = 0; t < T; ++t)
+  for (int t = 0; t < TK; ++t)
 #pragma unroll
-    for (int n = 0; n < T; ++n) {
-      const int k = k0 + 16 * (wk * T + t) + (OI ? i : 4 * g), c = n0 + 16 * (wn * T + n) + (OI ? 4 * g : i);
+    for (int n = 0; n < TN; ++n) {
+      const int k = k0 + 16 * (wk * TK + t) + (OI ? i : 4 * g), c = n0 + 16 * (wn * TN + n) + (OI ? 4 * g : i);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int kk = k + (OI ? 0 : r), cc = c + (OI ? r : 0);
@@ -223,16 +291,16 @@ __global__ __launch_bounds__(256, 1) void f8_wgrad_kernel(WGradArgs a) {
     }
 }
 
-template <int T, int S, bool F32>
+template <class Tile, bool F32>
 int run_tiles(mx_backend* b, const char* name, WGradArgs a, bool whole) {
-  constexpr int W = 32 * T, P = F32 ? 3 : 1, kLds = 2 * (1 + P) * S * W * 2;
+  constexpr int W = Tile::W, P = F32 ? 3 : 1, kLds = 2 * (1 + P) * Tile::S * W * 2;
   const int64_t tk = (a.K + W - 1) / W, tn = (a.N + W - 1) / W;
   if (tk * tn >= (int64_t)1 << 31) return set_error(MX_ERR_INVALID, "F8WeightGradient: more than 2^31 workgroups");
   a.tiles_n = (int)tn;
-  auto k = a.oi ? (whole ? f8_wgrad_kernel<T, S, F32, true, true> : f8_wgrad_kernel<T, S, F32, true, false>)
-                : (whole ? f8_wgrad_kernel<T, S, F32, false, true> : f8_wgrad_kernel<T, S, F32, false, false>);
+  auto k = a.oi ? (whole ? f8_wgrad_kernel<Tile, F32, true, true> : f8_wgrad_kernel<Tile, F32, true, false>)
+                : (whole ? f8_wgrad_kernel<Tile, F32, false, true> : f8_wgrad_kernel<Tile, F32, false, false>);
   MX_CHECK_HIP(hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
-  return launch(b, name, [&] { dispatch(k, dim3((unsigned)(tk * tn)), dim3(256), kLds, b->stream, a); });
+  return launch(b, name, [&] { dispatch(k, dim3((unsigned)(tk * tn)), dim3(Tile::kThreads), kLds, b->stream, a); });
 }
 
 enum class Plan { kF32, kBf16, kBf16Large };
@@ -256,12 +324,12 @@ const char* f8_wgrad_name(const F8WGradDesc& d) {
 int f8_wgrad_run(mx_backend* b, const F8WGradDesc& d) {
   if (d.K == 0 || d.N == 0) return MX_OK;
   const WGradArgs a{d.x, d.x_scale, d.dy, d.out, (int)d.M, (int)d.K, (int)d.N, (int)blocks(d.K), d.out_dt, d.oi, 0};
-  const bool whole = d.K % 16 == 0 && d.N % 8 == 0 && aligned16(d.x) && aligned16(d.dy);
+  const bool whole = d.K % 16 == 0 && d.N % 8 == 0 && d.K <= 1 << 24 && d.N <= 1 << 24 && aligned16(d.x) && aligned16(d.dy);
   const char* name = f8_wgrad_name(d);
   switch (plan_of(d)) {
-    case Plan::kF32: return run_tiles<4, 32, true>(b, name, a, whole);
-    case Plan::kBf16: return run_tiles<4, 64, false>(b, name, a, whole);
-    default: return run_tiles<8, 64, false>(b, name, a, whole);
+    case Plan::kF32: return run_tiles<Tile<2, 2, 4, 4, 32, 2>, true>(b, name, a, whole);
+    case Plan::kBf16: return run_tiles<Tile<2, 2, 4, 4, 64, 2>, false>(b, name, a, whole);
+    default: return run_tiles<Tile<4, 2, 4, 8, 64, 2>, false>(b, name, a, whole);
   }
 }
 

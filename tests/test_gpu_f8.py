@@ -324,7 +324,7 @@ def wgrad_want(x, xs, dy64, oi, out, dy_dt, pow2=True):
 
 
 WGRAD = [(0, 8, 8), (1, 1, 1), (1, 128, 200), (3, 129, 65), (31, 256, 128), (33, 130, 257), (64, 512, 384), (97, 1000, 333), (128, 256, 1024),
-         (333, 384, 272), (500, 640, 136), (1025, 264, 520)]
+         (333, 384, 272), (500, 640, 136), (1025, 264, 520), (65, 3600, 3488), (100, 3585, 3459)]
 
 
 @pytest.mark.parametrize("out", [F32, BF16])
