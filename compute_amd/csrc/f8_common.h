@@ -58,6 +58,25 @@ __device__ __forceinline__ u32x4 load16(const uint8_t* p, int64_t n) {
   return v;
 }
 
+// Four consecutive results from element `at`, of which the first n are in the row; vec: four are whole
+// and aligned.
+__device__ __forceinline__ void store4(void* out, int64_t at, int n, bool vec, int dt, const f32x4& v) {
+  if (vec) {
+    if (n <= 0) return;
+    if (dt == MX_DTYPE_FLOAT32) {
+      *(f32x4*)((float*)out + at) = v;
+    } else {
+      const f32x2 lo = {v[0], v[1]}, hi = {v[2], v[3]};
+      *(u32x2*)((uint16_t*)out + at) = u32x2{__builtin_bit_cast(uint32_t, __builtin_convertvector(lo, bf16x2)),
+                                             __builtin_bit_cast(uint32_t, __builtin_convertvector(hi, bf16x2))};
+    }
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (r < n) store_f(out, at + r, dt, v[r]);
+}
+
 // Workgroup barrier ordering LDS only: global loads in flight stay in flight.
 __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
