@@ -176,7 +176,7 @@ def run_dense(backend, x, xs, w, ws, oi, act, out, b=None, b_dt=F32):
 
 DENSE = [(1, 1, 1), (1, 128, 16), (3, 127, 65), (2, 129, 130), (1, 4096, 512), (5, 1000, 333), (16, 512, 256), (17, 384, 200),
          (33, 2048, 640), (64, 256, 1001), (97, 640, 272), (130, 1024, 128), (200, 136, 264), (256, 512, 512), (300, 1536, 384),
-         (1, 144, 32001), (16, 256, 4104), (257, 128, 257), (520, 272, 400)]
+         (1, 144, 32001), (16, 256, 4104), (257, 128, 257), (520, 272, 400), (3390, 144, 3600)]
 
 
 @pytest.mark.parametrize("out", [F32, BF16])
