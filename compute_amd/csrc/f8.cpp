@@ -184,7 +184,7 @@ int copy_name(const char* name, char* buf, size_t buflen) {
 
 int f8_dense_run(mx_backend* b, const F8DenseDesc& d) {
   if (d.M == 0 || d.N == 0) return MX_OK;
-  if (d.x_dt == MX_DTYPE_F8E4M3FN || d.K == 0) return f8_product_run(b, d);
+  if (d.x_dt == MX_DTYPE_F8E4M3FN || d.K == 0 || f8_product_takes_float(d)) return f8_product_run(b, d);
   // Codes, then scales on a 256-byte boundary, in one block.
   const size_t codes = ((size_t)d.M * d.K + 255) & ~(size_t)255;
   void* mem = nullptr;

@@ -48,6 +48,13 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
+// 16 bytes from any address.
+__device__ __forceinline__ u32x4 load16_any(const uint8_t* p) {
+  u32x4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+
 // 16 bytes from p, of which the first n are there (the rest 0).  p may be any byte.
 __device__ __forceinline__ u32x4 load16(const uint8_t* p, int64_t n) {
   u32x4 v = {0u, 0u, 0u, 0u};

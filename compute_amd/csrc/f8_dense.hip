@@ -18,43 +18,11 @@
 // result: column i, rows 4 g .. 4 g + 3.
 #include <algorithm>
 
-#include "f8_common.h"
-#include "mxrt_internal.h"
+#include "f8_dense.h"
 
 namespace mx {
 namespace {
 using namespace f8;
-
-struct DenseArgs {
-  const uint8_t* x;
-  const float* x_scale;
-  const uint8_t* w;
-  const float* w_scale;
-  const void* bias;
-  void* out;
-  int M, K, N, KB, NB;
-  int b_dt, out_dt, act, oi;
-  int tiles_n, vec_out;
-};
-
-__device__ __forceinline__ f32x4 mfma_f8(const i32x8& a, const i32x8& b, const f32x4& c) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
-}
-
-// The sum of products of one block.
-template <bool WIDE>
-__device__ __forceinline__ f32x4 block_sum(const i32x8& a, const i32x8& b) {
-  f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
-  if constexpr (WIDE) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8((uint32_t)a[2 * j], (uint32_t)a[2 * j + 1]),
-                                                  widen8((uint32_t)b[2 * j], (uint32_t)b[2 * j + 1]), t, 0, 0, 0);
-    return t;
-  } else {
-    return mfma_f8(a, b, t);
-  }
-}
 
 // Any sizes, alignment and layout: 64 x 64 tiles, both operands staged in LDS as rows of 128 codes.
 constexpr int kAnyTile = 64, kAnyThreads = 256, kAnyPitch = kBlock + 16;
@@ -411,9 +379,10 @@ int run_dense_tiles(mx_backend* b, const char* name, DenseArgs a) {
 using Tile256 = DenseTile<4, 2, 8>;  // 256 x 256
 using Tile128 = DenseTile<4, 2, 4>;  // 256 columns x 128 rows
 
-enum class DensePlan { kAny, kTiles256, kTiles128 };
+enum class DensePlan { kAny, kSkinny, kTiles256, kTiles128 };
 
 DensePlan dense_plan(const F8DenseDesc& d) {
+  if (skinny_fits(d)) return DensePlan::kSkinny;
   // The direct loads take whole aligned 16-byte chunks of rows and 32-bit offsets.
   const bool chunks = d.K % 16 == 0 && (d.oi || d.N % 16 == 0) && aligned16(d.x) && aligned16(d.w) && d.K <= 1 << 21 && d.N <= 1 << 21;
   if (!chunks || d.out_dt != MX_DTYPE_BFLOAT16 || d.K == 0) return DensePlan::kAny;
@@ -425,18 +394,21 @@ DensePlan dense_plan(const F8DenseDesc& d) {
 
 const char* f8_product_name(const F8DenseDesc& d) {
   switch (dense_plan(d)) {
+    case DensePlan::kSkinny: return "f8_dense_skinny";
     case DensePlan::kTiles256: return "f8_dense_tiles_256";
     case DensePlan::kTiles128: return "f8_dense_tiles_128";
     default: return "f8_dense_any";
   }
 }
 
+bool f8_product_takes_float(const F8DenseDesc& d) { return skinny_fits(d); }
+
 int f8_product_run(mx_backend* b, const F8DenseDesc& d) {
   if (d.M == 0 || d.N == 0) return MX_OK;
-  DenseArgs a{(const uint8_t*)d.x, d.x_scale, d.w, d.w_scale, d.bias, d.out, (int)d.M, (int)d.K, (int)d.N, (int)blocks(d.K),
-              (int)blocks(d.N), d.b_dt, d.out_dt, d.act, d.oi, 0, 0};
+  DenseArgs a = dense_args(d);
   const char* name = f8_product_name(d);
   switch (dense_plan(d)) {
+    case DensePlan::kSkinny: return skinny_run(b, d, name);
     case DensePlan::kTiles256:
     case DensePlan::kTiles128: {
       const bool large = dense_plan(d) == DensePlan::kTiles256;
