@@ -1,12 +1,12 @@
 // Dense product over 8-bit floating-point blocks for up to 16 rows (decode), weights [N, K].
 //
 // The weights are read once and are nearly all the bytes, so the work is to keep them coming: a workgroup
-// owns 16 columns, its waves take the blocks of 128 k in turn, and a wave keeps up to 2 kAhead blocks in flight
+// owns 16 or 32 columns (C operands of 16), its waves take the blocks of 128 k in turn, and a wave keeps up to 2 kAhead blocks in flight
 // straight into the registers that the MFMA reads (lane (i, g): 32 codes of column i from 32 g; 16 segments of
 // 128 bytes an instruction pair).  There is no LDS on the way, no
 // barrier before the end and nothing to share but x.  The waves' sums are added through LDS in wave order.
 //
-// [1, 4096] x [4096, 11008]: 45 MB.  See run_skinny for the measured times and the number of waves.
+// [1, 4096] x [4096, 11008] reads 45 MB in 10.7 us (4.2 TB/s; a large copy moves 4.9); run_skinny has more.
 //
 // x: codes with their scales, each lane (i, g) its own 32 codes of row i; or up to four rows of float values, which
 // each wave makes into codes for its own blocks, 16 lanes a row, as the quantiser does, and passes to the MFMA's
@@ -26,30 +26,35 @@ constexpr int kAhead = 2;        // blocks requested at once, with as many in fl
 constexpr int kFloatRows = 4;    // rows that a wave converts in one pass
 constexpr int kPitch = kBlock + 16;
 
-template <int X, bool WIDE, int NW>
+template <int X, bool WIDE, int NW, int C>
 __global__ __launch_bounds__(64 * NW) void f8_skinny_kernel(DenseArgs a) {
   constexpr bool kFloat = X != kCodes;
   __shared__ __align__(16) uint8_t codes[kFloat ? NW : 1][kFloat ? kFloatRows * kPitch : 16];
   __shared__ float scales[kFloat ? NW : 1][kFloatRows];
-  __shared__ f32x4 sums[NW][64];
+  __shared__ f32x4 sums[NW][C][64];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), i = lane % 16, g = lane / 16;
-  const int n0 = 16 * xcd_order((int)blockIdx.x, (int)gridDim.x);
-  const uint8_t* wrow = a.w + (int64_t)min(n0 + i, a.N - 1) * a.K + 32 * g;
+  const int n0 = 16 * C * xcd_order((int)blockIdx.x, (int)gridDim.x);
+  const uint8_t* wrow[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) wrow[c] = a.w + (int64_t)min(n0 + 16 * c + i, a.N - 1) * a.K + 32 * g;
   const uint8_t* xrow = a.x + (int64_t)min(i, a.M - 1) * a.K + 32 * g;
   const float* sw = a.w_scale + (int64_t)(n0 / kBlock) * a.KB;
   const bool row = i < a.M;
   const int fr = g, fk = 8 * i;  // float x: the lane's row and first value of a block
 
   struct Block {
-    u32x4 w[2], x[X == kBf16 ? 1 : 2];
+    u32x4 w[C][2], x[X == kBf16 ? 1 : 2];
     float sw, sx;
   };
   auto request = [&](int kb, bool whole) __attribute__((always_inline)) {
     Block o;
     const int k = kb * kBlock, left = a.K - k;  // whole: at least a block
     auto load = [&](const uint8_t* p, int n) __attribute__((always_inline)) { return whole ? load16_any(p) : load16(p, n); };
-    o.w[0] = load(wrow + k, left - 32 * g);
-    o.w[1] = load(wrow + k + 16, left - 32 * g - 16);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      o.w[c][0] = load(wrow[c] + k, left - 32 * g);
+      o.w[c][1] = load(wrow[c] + k + 16, left - 32 * g - 16);
+    }
     o.sw = sw[kb];
     o.x[0] = u32x4{0u, 0u, 0u, 0u};
     if constexpr (X != kBf16) o.x[1] = o.x[0];
@@ -109,14 +114,17 @@ __global__ __launch_bounds__(64 * NW) void f8_skinny_kernel(DenseArgs a) {
     }
   };
 
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 acc[C] = {};
   auto multiply = [&](const Block& blk) __attribute__((always_inline)) {
     float sx;
     const i32x8 xo = operand(blk, sx);
-    const f32x4 t = block_sum<WIDE>(join(blk.w[0], blk.w[1]), xo);
     const float sc = sx * blk.sw;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) acc[r] = fmaf(t[r], sc, acc[r]);
+    for (int c = 0; c < C; ++c) {
+      const f32x4 t = block_sum<WIDE>(join(blk.w[c][0], blk.w[c][1]), xo);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[c][r] = fmaf(t[r], sc, acc[c][r]);
+    }
   };
   // Whole blocks wave, wave + NW, ..: groups of kAhead, the next requested before the present is multiplied.
   const int whole = a.K / kBlock, mine = whole > wave ? (whole - wave + NW - 1) / NW : 0;
@@ -139,26 +147,41 @@ __global__ __launch_bounds__(64 * NW) void f8_skinny_kernel(DenseArgs a) {
     products(1, first + kAhead);
   }
   if (whole < a.KB && wave == whole % NW) multiply(request(whole, false));  // the short last block
-  sums[wave][lane] = acc;
+#pragma unroll
+  for (int c = 0; c < C; ++c) sums[wave][c][lane] = acc[c];
   __syncthreads();
-  for (int o = threadIdx.x; o < 16 * a.M; o += 64 * NW) {
-    const int m = o / 16, n = o % 16;
+  for (int o = threadIdx.x; o < 16 * C * a.M; o += 64 * NW) {
+    const int m = o / (16 * C), n = o % (16 * C);
     if (n0 + n >= a.N) continue;
     float v = 0.0f;
 #pragma unroll
-    for (int q = 0; q < NW; ++q) v += sums[q][16 * (n / 4) + m][n % 4];
+    for (int q = 0; q < NW; ++q) v += sums[q][n / 16][16 * (n % 16 / 4) + m][n % 4];
     if (a.bias) v += load_f(a.bias, n0 + n, a.b_dt);
     store_f(a.out, (int64_t)m * a.N + n0 + n, a.out_dt, act_fast(v, a.act));
   }
 }
 
+// Waves of a workgroup and operands of columns.  Measured (us, bf16 results; waves x operands 4x1, 4x2, 8x1, 16x1):
+//   one bf16 row   [4096] x 11008   10.7  12.6  10.9  12.1      16 rows  [2048] x 32001, f32   20.0  16.0  21.0  29.2
+//                  [4096] x 4096     7.8   8.3   5.8   5.3               [4096] x 14336         19.6  15.8  19.3  21.6
+//                  [14336] x 4096   18.6  21.0  12.4  12.0               [4096] x 4096           8.5   9.6   7.1   8.2
+//                                                              8 rows    [14336] x 4096         15.1  20.7  14.0  14.2
+// From 768 strips the CUs are full with two operands, which share the lanes' x (as many bytes as the weights with 16
+// rows); from 512 with four waves; below, the waves have to come from K, and their sums cost the rows of codes more.
 template <int X, bool WIDE>
 int run_skinny(mx_backend* b, const char* name, const DenseArgs& a) {
-  const int strips = (a.N + 15) / 16;
-  auto go = [&](auto k, int waves) {
+  auto go = [&](auto k, int waves, int c) {
+    const int strips = (int)(((int64_t)a.N + 16 * c - 1) / (16 * c));
     return launch(b, name, [&] { dispatch(k, dim3((unsigned)strips), dim3(64 * waves), 0, b->stream, a); });
   };
-  return strips >= 256 ? go(f8_skinny_kernel<X, WIDE, 8>, 8) : go(f8_skinny_kernel<X, WIDE, 16>, 16);
+  const int strips = (int)(((int64_t)a.N + 15) / 16);
+  if constexpr (X == kCodes) {
+    if (strips >= 768) return go(f8_skinny_kernel<X, WIDE, 4, 2>, 4, 2);
+    if (strips < 512) return go(f8_skinny_kernel<X, WIDE, 8, 1>, 8, 1);
+  } else {
+    if (strips < 512) return go(f8_skinny_kernel<X, WIDE, 16, 1>, 16, 1);
+  }
+  return go(f8_skinny_kernel<X, WIDE, 4, 1>, 4, 1);
 }
 
 }  // namespace

@@ -176,7 +176,7 @@ def run_dense(backend, x, xs, w, ws, oi, act, out, b=None, b_dt=F32):
 
 DENSE = [(1, 1, 1), (1, 128, 16), (3, 127, 65), (2, 129, 130), (1, 4096, 512), (5, 1000, 333), (16, 512, 256), (17, 384, 200),
          (33, 2048, 640), (64, 256, 1001), (97, 640, 272), (130, 1024, 128), (200, 136, 264), (256, 512, 512), (300, 1536, 384),
-         (1, 144, 32001), (16, 256, 4104), (257, 128, 257), (520, 272, 400), (3390, 144, 3600)]
+         (1, 144, 32001), (16, 256, 4104), (257, 128, 257), (520, 272, 400), (3390, 144, 3600), (5, 200, 9001)]
 
 
 @pytest.mark.parametrize("out", [F32, BF16])
@@ -197,7 +197,7 @@ def test_dense_epilogue(backend, M, K, N, oi, b_dt, out, act):
     assert_within(run_dense(backend, x, xs, w, ws, oi, act, out, b, b_dt), want, bound, f"act {act}")
 
 
-@pytest.mark.parametrize("M,K,N,dt", [(1, 4096, 256, BF16), (3, 300, 200, F32), (16, 1024, 320, BF16), (40, 384, 272, F32), (300, 512, 256, BF16),
+@pytest.mark.parametrize("M,K,N,dt", [(1, 4096, 256, BF16), (2, 300, 8200, BF16), (4, 2500, 40, F32), (3, 300, 200, F32), (16, 1024, 320, BF16), (40, 384, 272, F32), (300, 512, 256, BF16),
                                       (0, 256, 128, F32)])
 def test_dense_of_float_x(backend, M, K, N, dt):
     """Float x is what its codes and scales are: the same bits as quantising first; its dtype is the default output's."""
