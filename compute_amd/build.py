@@ -26,7 +26,7 @@ COMMON = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 SOURCES = ["runtime.cpp", "graph.cpp", "qdense.hip", "qdense_skinny.hip", "qdense_gemv.hip", "qdense_gemm.hip", "qdense_refgemm.hip", "qdense_refgemm_bf16.hip", "qdense_noalloc.hip", "ggml.hip", "dot.hip", "elementwise.hip",
-           "f8.cpp", "f8_elementwise.hip", "f8_dense.hip", "f8_skinny.hip", "f8_wgrad.hip"]
+           "f8.cpp", "f8_elementwise.hip", "f8_dense.hip", "f8_dense_staged.hip", "f8_skinny.hip", "f8_wgrad.hip"]
 
 
 # The skinny kernel takes one arrival ticket per workgroup from a single lane; LLVM's atomic

@@ -18,6 +18,9 @@ struct DenseArgs {
   int M, K, N, KB, NB;
   int b_dt, out_dt, act, oi;
   int tiles_n, vec_out;
+  int S, kps;         // slices of K of a tile, blocks of a slice
+  char* part;         // [tile][slice] sums (S > 1)
+  uint32_t* arrived;  // [tile], zero between launches
 };
 
 __device__ __forceinline__ f32x4 mfma_f8(const i32x8& a, const i32x8& b, const f32x4& c) {
@@ -42,12 +45,14 @@ __device__ __forceinline__ f32x4 block_sum(const i32x8& a, const i32x8& b) {
 inline DenseArgs dense_args(const F8DenseDesc& d) {
   const bool codes = d.x_dt == MX_DTYPE_F8E4M3FN;
   return DenseArgs{codes ? (const uint8_t*)d.x : nullptr, codes ? nullptr : d.x, d.x_scale, d.w, d.w_scale, d.bias, d.out,
-                   (int)d.M, (int)d.K, (int)d.N, (int)blocks(d.K), (int)blocks(d.N), d.b_dt, d.out_dt, d.act, d.oi, 0, 0};
+                   (int)d.M, (int)d.K, (int)d.N, (int)blocks(d.K), (int)blocks(d.N), d.b_dt, d.out_dt, d.act, d.oi, 0, 0, 1, 0, nullptr, nullptr};
 }
 
 // Up to 16 rows, weights [N, K] (f8_skinny.hip); float x up to four rows.
 bool skinny_fits(const F8DenseDesc& d);
 int skinny_run(mx_backend* b, const F8DenseDesc& d, const char* name);
+// Tiles whose operands come through registers (f8_dense_staged.hip).
+int staged_run(mx_backend* b, const char* name, const DenseArgs& a, bool wide, int tile, int slices);
 
 }  // namespace f8
 }  // namespace mx

@@ -1,0 +1,491 @@
+// Dense product over 8-bit floating-point blocks:
+//   y[m, n] = act(sum_b sx[m, b] * sw[b, n / 128] * (sum_{k in block b} x[m, k] * w[k, n]) + bias[n]).
+//
+// A block of 128 codes is one v_mfma_f32_16x16x128_f8f6f4, whose sum starts from zero and enters the
+// float32 total with the block's two scales: acc += t * (sx * sw).
+//
+// Precision.  The matrix cores add the products of 8-bit operands in groups of eight, aligned to the
+// group's largest and cut off 13 bits below it (measured with single products, for every 8-bit form
+// of the instruction); groups are added in float32.  On random codes of mixed exponents a sum of 128
+// is 4.4e-5 off in norm.  That is 1/38 of the rounding of a bfloat16 result, which therefore takes
+// these instructions at 4.4 PFLOP/s.  A float32 result (WIDE) takes the codes as bfloat16 values, which
+// are exact, through v_mfma_f32_16x16x32_bf16, whose sums are good to 2^-23 of their terms, at half the
+// rate.
+//
+// Operand layout.  Lane (i = lane % 16, g = lane / 16) of the instruction holds 32 consecutive codes of
+// row (or column) i, those from 32 g; the sum does not depend on which k a position stands for as
+// long as both operands agree.  WIDE: four instructions, each over eight of a lane's 32 codes.  The
+// result: column i, rows 4 g .. 4 g + 3.
+#pragma once
+
+#include <algorithm>
+
+#include "f8_dense.h"
+
+namespace mx {
+namespace f8 {
+namespace {
+
+// -------------------------------------------------------------------------------------------------
+// Tiles.  A workgroup of WN x WM waves computes 64 WN columns (n) x 16 TB WM rows (m), a wave
+// 64 x 16 TB of it, one block of 128 k a step.
+//
+// Roles.  w is the first operand, so that a lane's four results of a tile are four columns of one row: the scale
+// of a tile is then one value a lane, sx of its row times the wave's sw.
+//
+// Staging.  Codes and scales move from memory straight into LDS (buffer_load ... lds, 16 or 4 bytes a lane), BUF
+// steps ahead, into BUF buffers.  The resources end with their arrays, and past the end LDS gets zeros: rows past M or N and,
+// for w [K, N], rows past K need nothing more.  The last block's chunks past K are sent past the end by their offset.
+//   x, and w [N, K] (OI): rows of 128 bytes.  A lane reads its 32 codes as two 16-byte chunks; chunk c of row r lies at
+//     c ^ (r >> 1 & 7) for x, whose operands are 16 consecutive rows, and at c ^ ((r >> 1 & 1) | (r >> 4 & 3) << 1) for
+//     w: operand a of a wave is the rows 16 (i / 4) + 4 a + i % 4 of its 64, which leaves a lane with 16 consecutive
+//     columns over its four operands.  Either way 16 lanes meet every bank once.
+//   DMA: these loads take whole aligned chunks and 32-bit offsets.  Otherwise the chunks come through registers, from
+//     any address, requested a step ahead and written to the same places of two buffers.
+//   w [K, N] (!OI): 128 rows of k, 64 WN columns, read through the transposing read, eight k at a time; 16-byte chunk c
+//     of row k lies at c ^ k_swizzle(k), which sends the 8 rows and two halves of 16 lanes to all banks.
+//
+// Schedule.  A step is TB groups of four MFMAs, one operand of x against the wave's four of w.  An operand of x is
+// read kRing - 1 groups ahead; a group's sums enter the total during the next group.  The step's barrier stands before
+// its last kRing - 1 groups, whose operands are in registers: behind it the step BUF ahead is requested into the
+// buffer just left, and w's operands are read again as the last group leaves them.
+struct Resource {
+  i32x4 d;
+};
+__device__ __forceinline__ Resource make_resource(const void* p, int64_t bytes) {
+  constexpr int64_t kMost = 0x7fffffff;  // offsets from 2^31 on are past the end
+  const uint64_t at = (uint64_t)(uintptr_t)p;
+  return Resource{i32x4{(int)(uint32_t)at, (int)((uint32_t)(at >> 32) & 0xffffu), (int)(bytes < 0 ? 0 : bytes < kMost ? bytes : kMost), 0x00027000}};
+}
+constexpr uint32_t kPastEnd = 0x80000000u;
+
+// 16 (or 4) bytes a lane from offset voff of a resource, lane l's to LDS address `to` + 16 l (4 l); past the
+// resource's end zeros.  Issued as assembly: the compiler neither waits for it nor knows that it writes LDS, so the
+// kernel waits itself (wait_loads) before the barrier that publishes a step, and before it ends.
+__device__ __forceinline__ void lds_load16(const Resource& r, uint32_t voff, uint32_t to) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(voff), "s"(to), "s"(r.d)
+      : "memory");
+}
+__device__ __forceinline__ void lds_load4(const Resource& r, uint32_t voff, uint32_t to) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %1, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(voff), "s"(to), "s"(r.d)
+      : "memory");
+}
+// Until at most N of the wave's loads are in flight.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+}
+
+typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) const float lds_float;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4_rw;
+typedef __attribute__((address_space(3))) float lds_float_rw;
+__device__ __forceinline__ u32x4 lds_read16(uint32_t at) { return *(lds_u32x4*)at; }
+__device__ __forceinline__ float lds_read_float(uint32_t at) { return *(lds_float*)at; }
+
+// The first n bytes of v, the rest 0.
+__device__ __forceinline__ u32x4 first_bytes(u32x4 v, int n) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int left = n - 4 * e;
+    v[e] = left >= 4 ? v[e] : left <= 0 ? 0u : v[e] & ((1u << (8 * left)) - 1u);
+  }
+  return v;
+}
+
+template <int WN_, int WM_, int TB_, int BUF_>
+struct DenseTile {
+  static constexpr int WN = WN_, WM = WM_, TB = TB_, BUF = BUF_, kWaves = WN * WM, kThreads = 64 * kWaves;
+  static constexpr int kCols = 64 * WN, kRows = 16 * TB * WM;
+  static constexpr int kXBytes = kRows * kBlock, kWBytes = kCols * kBlock, kScaleBytes = 4 * kRows + 256;
+  static constexpr int kX = 0, kW = BUF * kXBytes, kScale = kW + BUF * kWBytes, kLds = kScale + BUF * kScaleBytes;
+  static constexpr int kLoads = kXBytes / (1024 * kWaves) + kWBytes / (1024 * kWaves) + 1;  // of a wave a step
+  static constexpr int kPartBytes = 4 * kRows * kCols;
+  // 16-byte chunk c of row k of w [K, N] lies at c ^ k_swizzle(k).
+  static constexpr int kShift = kCols == 256 ? 0 : kCols == 128 ? 1 : 2;
+  static __device__ __forceinline__ int k_swizzle(int k) { return 2 * ((k >> kShift) & (7 >> kShift)) | (k >> 5 & 1); }
+  static_assert(kXBytes % (1024 * kWaves) == 0 && kWBytes % (1024 * kWaves) == 0, "whole loads");
+  static_assert(kRows % 64 == 0 && kRows / 64 < kWaves, "a wave a load of row scales, and one of the weight's");
+};
+
+// A wave's results: lane (i, g) has, of each row 16 b + i, 16 consecutive columns from 16 g (OI) or four from 16 c + 4 g.
+template <int ACT, bool OI, bool F32, int TB>
+__device__ __forceinline__ void store_results(const DenseArgs& a, const f32x4 (&acc)[4][TB], int m0, int n0) {
+  const int lane = threadIdx.x % 64, i = lane % 16, g = lane / 16;
+  float bias[4][4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int n = n0 + (OI ? 16 * g + 4 * c : 16 * c + 4 * g) + r;
+      bias[c][r] = a.bias && n < a.N ? load_f(a.bias, n, a.b_dt) : 0.0f;
+    }
+#pragma unroll
+  for (int b = 0; b < TB; ++b) {
+    const int m = m0 + 16 * b + i;
+    if (m >= a.M) continue;
+    f32x4 v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[c][r] = act_fast(acc[c][b][r] + bias[c][r], ACT);
+    const int64_t row = (int64_t)m * a.N;
+    if (OI && !F32 && a.vec_out) {  // rows on 16 bytes, N a multiple of 8
+      u32x4 o[2];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          const f32x2 p = {v[c][r], v[c][r + 1]};
+          o[c / 2][2 * (c % 2) + r / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf16x2));
+        }
+      const int n = n0 + 16 * g;
+      uint16_t* to = (uint16_t*)a.out + row + n;
+      if (n < a.N) *(u32x4*)to = o[0];
+      if (n + 8 < a.N) *(u32x4*)(to + 8) = o[1];
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int n = n0 + (OI ? 16 * g + 4 * c : 16 * c + 4 * g);
+        store4(a.out, row + n, a.N - n, a.vec_out, F32 ? MX_DTYPE_FLOAT32 : MX_DTYPE_BFLOAT16, v[c]);
+      }
+    }
+  }
+}
+
+// An operand of the MFMA: 32 codes, or (WIDE) the bf16 values of eight at a time.
+template <bool WIDE>
+struct Operand {
+  i32x8 v;
+  __device__ __forceinline__ void set(const i32x8& codes) { v = codes; }
+};
+template <>
+struct Operand<true> {
+  bf16x8 v[4];
+  __device__ __forceinline__ void set(const i32x8& c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = widen8((uint32_t)c[2 * j], (uint32_t)c[2 * j + 1]);
+  }
+};
+__device__ __forceinline__ f32x4 block_sum(const Operand<false>& a, const Operand<false>& b) {
+  return mfma_f8(a.v, b.v, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+}
+__device__ __forceinline__ f32x4 block_sum(const Operand<true>& a, const Operand<true>& b) {
+  f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[j], b.v[j], t, 0, 0, 0);
+  return t;
+}
+
+template <class Tile, bool OI, bool WIDE, bool DMA>
+__global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(DenseArgs a) {
+  constexpr int TB = Tile::TB, kWaves = Tile::kWaves;
+  constexpr int kRing = 2, kLast = kRing - 1;
+  constexpr int XL = Tile::kXBytes / (1024 * kWaves), WL = Tile::kWBytes / (1024 * kWaves);  // loads a wave a step
+  static_assert(TB % kRing == 0, "the ring's slots are the same in every step");
+  extern __shared__ __align__(1024) uint8_t lds[];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), i = lane % 16, g = lane / 16;
+  const uint32_t base = lds_addr(lds);
+  int mt, nt, tile, slice;
+  {
+    // Runs of 4 tiles of n by all tiles of m: a run's workgroups share their rows of x and w in an L2.  A tile's
+    // slices are neighbours.
+    const int tiles = (int)gridDim.x / a.S, tiles_m = tiles / a.tiles_n;
+    const int it = xcd_order((int)blockIdx.x, (int)gridDim.x);
+    const int t = it / a.S;
+    tile = t;
+    slice = it - t * a.S;
+    const int per = 4 * tiles_m, q = t / per, cols = min(4, a.tiles_n - 4 * q), in = t - q * per;
+    nt = 4 * q + in % cols;
+    mt = in / cols;
+  }
+  const int m0 = mt * Tile::kRows, n0 = nt * Tile::kCols;
+
+  // Loads: the wave's lanes' offsets within a step, and what moves with it.
+  uint32_t x_off[XL], w_off[WL], x_tail[XL], w_tail[WL];
+  const int last = a.K - (a.KB - 1) * kBlock;  // codes of the last block
+#pragma unroll
+  for (int j = 0; j < XL; ++j) {
+    const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ (r >> 1 & 7);
+    x_off[j] = (uint32_t)r * (uint32_t)a.K + 16 * c;
+    x_tail[j] = 16 * c >= last ? kPastEnd : 0u;
+  }
+  constexpr int kLanesRow = Tile::kCols / 16;  // !OI: lanes of a row of k
+#pragma unroll
+  for (int j = 0; j < WL; ++j) {
+    if constexpr (OI) {
+      const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ ((r >> 1 & 1) | (r >> 4 & 3) << 1);
+      w_off[j] = (uint32_t)r * (uint32_t)a.K + 16 * c;
+      w_tail[j] = 16 * c >= last ? kPastEnd : 0u;
+    } else {
+      const int k = (64 / kLanesRow) * (wave + kWaves * j) + lane / kLanesRow;
+      w_off[j] = (uint32_t)k * (uint32_t)a.N + 16 * ((lane % kLanesRow) ^ Tile::k_swizzle(k));
+      w_tail[j] = 0u;
+    }
+  }
+  const uint8_t* xp = a.x + (int64_t)m0 * a.K;
+  const int64_t x_left = (int64_t)(a.M - m0) * a.K;
+  const uint8_t* wp = OI ? a.w + (int64_t)n0 * a.K : a.w + n0;
+  const int64_t w_left = OI ? (int64_t)(a.N - n0) * a.K : (int64_t)a.K * a.N - n0;
+  // Waves below kRows / 64 load 64 row scales each, the others (all the same) the weight's of the tile's columns.
+  const bool row_scales = wave < Tile::kRows / 64;
+  const uint8_t* sp = (const uint8_t*)(row_scales ? a.x_scale + (int64_t)(m0 + 64 * wave) * a.KB : a.w_scale);
+  const int64_t s_left = 4 * (row_scales ? (int64_t)(a.M - m0 - 64 * wave) * a.KB : (int64_t)a.KB * a.NB);
+  const uint32_t nb = (uint32_t)min(n0 / kBlock + lane % ((Tile::kCols + kBlock - 1) / kBlock), a.NB - 1);
+  const uint32_t s_off = 4 * (row_scales ? (uint32_t)lane * (uint32_t)a.KB : OI ? nb * (uint32_t)a.KB : nb);
+  const uint32_t s_step = row_scales || OI ? 4 : 4 * (uint32_t)a.NB;
+  const uint32_t s_to = base + Tile::kScale + (row_scales ? 256 * wave : 4 * Tile::kRows);
+  if constexpr (!DMA) static_assert(Tile::BUF == 2, "the buffers alternate");
+  u32x4 xg[XL], wg[WL];
+  float sg = 0.0f;
+  const int64_t x_total = (int64_t)a.M * a.K, w_total = (int64_t)a.K * a.N;
+  auto fetch = [&](int block) __attribute__((always_inline)) {  // !DMA: a block's chunks into registers
+    const int kb = min(block, a.KB - 1);
+    // Away from the arrays' ends a chunk may run on into the next row.
+    const bool x_inside = (int64_t)(a.M - m0 - Tile::kRows) * a.K >= 16;
+    const bool w_inside = OI ? (int64_t)(a.N - n0 - Tile::kCols) * a.K >= 16 : (int64_t)(a.K - (kb + 1) * kBlock) * a.N >= 16;
+#pragma unroll
+    for (int j = 0; j < XL; ++j) {
+      const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ (r >> 1 & 7);
+      const int64_t at = (int64_t)min(m0 + r, a.M - 1) * a.K + min(kb * kBlock + 16 * c, a.K - 1);
+      xg[j] = x_inside ? load16_any(a.x + at) : load16(a.x + at, x_total - at);
+    }
+#pragma unroll
+    for (int j = 0; j < WL; ++j) {
+      int64_t at;
+      if constexpr (OI) {
+        const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ ((r >> 1 & 1) | (r >> 4 & 3) << 1);
+        at = (int64_t)min(n0 + r, a.N - 1) * a.K + min(kb * kBlock + 16 * c, a.K - 1);
+      } else {
+        const int k = (64 / kLanesRow) * (wave + kWaves * j) + lane / kLanesRow;
+        at = (int64_t)min(kb * kBlock + k, a.K - 1) * a.N + min(n0 + 16 * ((lane % kLanesRow) ^ Tile::k_swizzle(k)), a.N - 1);
+      }
+      wg[j] = w_inside ? load16_any(a.w + at) : load16(a.w + at, w_total - at);
+    }
+    const int row = min(m0 + 64 * wave + lane, a.M - 1);
+    sg = row_scales ? a.x_scale[(int64_t)row * a.KB + kb] : OI ? a.w_scale[(int64_t)nb * a.KB + kb] : a.w_scale[(int64_t)kb * a.NB + nb];
+  };
+  auto stage = [&](int block, uint32_t buf) __attribute__((always_inline)) {  // !DMA: and on into LDS
+    if (block >= a.KB - 1 && last < kBlock) {  // the short last block: nothing past K
+#pragma unroll
+      for (int j = 0; j < XL; ++j) {
+        const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ (r >> 1 & 7);
+        xg[j] = first_bytes(xg[j], last - 16 * c);
+      }
+#pragma unroll
+      for (int j = 0; j < WL; ++j) {
+        if constexpr (OI) {
+          const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ ((r >> 1 & 1) | (r >> 4 & 3) << 1);
+          wg[j] = first_bytes(wg[j], last - 16 * c);
+        } else {
+          const int k = (64 / kLanesRow) * (wave + kWaves * j) + lane / kLanesRow;
+          if (k >= last) wg[j] = u32x4{0u, 0u, 0u, 0u};
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < XL; ++j) *(lds_u32x4_rw*)(base + Tile::kX + buf * Tile::kXBytes + 1024 * (wave + kWaves * j) + 16 * lane) = xg[j];
+#pragma unroll
+    for (int j = 0; j < WL; ++j) *(lds_u32x4_rw*)(base + Tile::kW + buf * Tile::kWBytes + 1024 * (wave + kWaves * j) + 16 * lane) = wg[j];
+    *(lds_float_rw*)(s_to + buf * Tile::kScaleBytes + 4 * lane) = sg;
+  };
+  // DMA: the last block's chunks past K are sent past the end.  (Blocks past the last are requested like any other, from
+  // wherever they lie, and not used.)
+  auto request = [&](int kb, uint32_t buf) __attribute__((always_inline)) {
+    const Resource xr = make_resource(xp + (int64_t)kb * kBlock, x_left - (int64_t)kb * kBlock);
+    const Resource sr = make_resource(sp + (int64_t)kb * s_step, s_left - (int64_t)kb * s_step);
+    const uint32_t in_last = kb == a.KB - 1 ? 0xffffffffu : 0u;
+#pragma unroll
+    for (int j = 0; j < XL; ++j)
+      lds_load16(xr, x_off[j] | (x_tail[j] & in_last), base + Tile::kX + buf * Tile::kXBytes + 1024 * (wave + kWaves * j));
+    const int64_t moved = (int64_t)kb * kBlock * (OI ? 1 : a.N);
+    const Resource wr = make_resource(wp + moved, w_left - moved);
+#pragma unroll
+    for (int j = 0; j < WL; ++j)
+      lds_load16(wr, w_off[j] | (w_tail[j] & in_last), base + Tile::kW + buf * Tile::kWBytes + 1024 * (wave + kWaves * j));
+    lds_load4(sr, s_off, s_to + buf * Tile::kScaleBytes);
+  };
+
+  // Operand reads.
+  const int wn = wave / Tile::WM, wm = wave % Tile::WM;
+  const int x_row = 16 * TB * wm + i, x_first = (2 * g) ^ (i >> 1 & 7);
+  const uint32_t xa = base + Tile::kX + x_row * kBlock + 16 * x_first;
+  uint32_t wa;
+  if constexpr (OI) {
+    const int r = 64 * wn + 16 * (i / 4) + i % 4, first = (2 * g) ^ ((i % 4) / 2 | (i / 4) << 1);
+    wa = base + Tile::kW + r * kBlock + 16 * first;
+  } else {
+    const int k = 32 * g + i / 2;
+    wa = base + Tile::kW + k * Tile::kCols + 16 * ((4 * wn) ^ Tile::k_swizzle(k)) + 8 * (i % 2);
+  }
+  const uint32_t sxa = base + Tile::kScale + 4 * x_row, swa = base + Tile::kScale + 4 * Tile::kRows + 4 * (64 * wn / kBlock);
+  i32x8 wo[4], xo[kRing];
+  float sx[kRing];
+  auto read_w = [&](int c, uint32_t buf) __attribute__((always_inline)) {
+    const uint32_t at = wa + buf * Tile::kWBytes;
+    if constexpr (OI) {
+      wo[c] = join(lds_read16(at + 4 * kBlock * c), lds_read16((at ^ 16) + 4 * kBlock * c));
+    } else {
+      const uint32_t p = at ^ (uint32_t)(16 * c);
+      const u32x2 k0 = read_tr8(p), k1 = read_tr8(p + 8 * Tile::kCols), k2 = read_tr8(p + 16 * Tile::kCols), k3 = read_tr8(p + 24 * Tile::kCols);
+      wo[c] = i32x8{(int)k0[0], (int)k0[1], (int)k1[0], (int)k1[1], (int)k2[0], (int)k2[1], (int)k3[0], (int)k3[1]};
+    }
+  };
+  auto read_x = [&](int b, uint32_t buf) __attribute__((always_inline)) {
+    const uint32_t at = xa + buf * Tile::kXBytes;
+    xo[b % kRing] = join(lds_read16(at + 16 * kBlock * b), lds_read16((at ^ 16) + 16 * kBlock * b));
+    sx[b % kRing] = lds_read_float(sxa + buf * Tile::kScaleBytes + 64 * b);
+  };
+
+  f32x4 acc[4][TB] = {}, t[2][4] = {};
+  Operand<WIDE> wv[4];
+  float st[2] = {};
+  const int kb0 = slice * a.kps, kb1 = min(a.KB, kb0 + a.kps);  // the slice's blocks
+  {
+    if constexpr (DMA) {
+#pragma unroll
+      for (int j = 0; j < Tile::BUF; ++j) request(kb0 + j, j);
+      wait_loads<(Tile::BUF - 1) * Tile::kLoads>();
+    } else {
+      fetch(kb0);
+      stage(kb0, 0);
+      fetch(kb0 + 1);
+    }
+    lds_barrier();
+    float sw = lds_read_float(swa);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) read_w(c, 0);
+#pragma unroll
+    for (int b = 0; b < kLast; ++b) read_x(b, 0);
+    uint32_t cur = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const uint32_t next = cur + 1 == Tile::BUF ? 0 : cur + 1;
+      float sw_next = 0.0f;
+#pragma unroll
+      for (int b = 0; b < TB; ++b) {
+        if (b == TB - kLast) {
+          if constexpr (DMA) {
+            wait_loads<(Tile::BUF - 2) * Tile::kLoads>();
+            lds_barrier();
+            request(kb + Tile::BUF, cur);
+          } else {
+            stage(kb + 1, next);
+            lds_barrier();
+            fetch(kb + 2);
+          }
+          sw_next = lds_read_float(swa + next * Tile::kScaleBytes);
+        }
+        if (b + kLast < TB)
+          read_x(b + kLast, cur);
+        else
+          read_x(b + kLast - TB, next);
+        st[b % 2] = sx[b % kRing] * sw;
+        if (b == 0) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) wv[c].set(wo[c]);
+        }
+        Operand<WIDE> xv;
+        xv.set(xo[b % kRing]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          t[b % 2][c] = block_sum(wv[c], xv);
+          if (b == TB - 1) read_w(c, next);
+        }
+        constexpr int kBefore = TB - 1;
+        const int p = b == 0 ? kBefore : b - 1;  // the group before (of the step before: t starts as zeros)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[c][p][r] = fmaf(t[1 - b % 2][c][r], st[1 - b % 2], acc[c][p][r]);
+#pragma unroll
+        for (int c = 0; c < (WIDE ? 16 : 4); ++c) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS read
+          __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // VALU
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      sw = sw_next;
+      cur = next;
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[c][TB - 1][r] = fmaf(t[1][c][r], st[1], acc[c][TB - 1][r]);
+    if constexpr (DMA) wait_loads<0>();  // of the blocks past the last: LDS is the next workgroup's when this one ends
+  }
+  static_assert(TB % 2 == 0, "the last group's sums lie in t[1]");
+  if (a.S > 1) {
+    // The slices' sums meet in scratch, stored and loaded with the agent-scope coherence bit (sc1): the slices may run
+    // on different XCDs.  The last to arrive adds them in order and goes on; it leaves the counter at zero.
+    __shared__ int s_last;
+    constexpr int kSc1 = 16;
+    const __amdgpu_buffer_rsrc_t prs = __builtin_amdgcn_make_buffer_rsrc((char*)a.part + (int64_t)tile * a.S * Tile::kPartBytes, 0,
+                                                                         a.S * Tile::kPartBytes, 0x00027000);
+    auto at = [&](int sl, int c, int b) { return (uint32_t)(sl * Tile::kPartBytes + ((c * TB + b) * Tile::kThreads + (int)threadIdx.x) * 16); };
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int b = 0; b < TB; ++b)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[c][b]), prs, at(slice, c, b), 0, kSc1);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const uint32_t before = __hip_atomic_fetch_add(&a.arrived[tile], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_last = before + 1u == (uint32_t)a.S;
+      if (s_last) __hip_atomic_store(&a.arrived[tile], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!s_last) return;
+#pragma unroll 1
+    for (int sl = 0; sl < a.S; ++sl)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int b = 0; b < TB; ++b) {
+          const f32x4 o = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(prs, at(sl, c, b), 0, kSc1));
+          acc[c][b] = sl == 0 ? o : acc[c][b] + o;
+        }
+  }
+  const int mw = m0 + 16 * TB * wm, nw = n0 + 64 * wn;
+  switch (a.act) {
+    case MX_ACT_GELU: store_results<MX_ACT_GELU, OI, WIDE, TB>(a, acc, mw, nw); break;
+    case MX_ACT_RELU: store_results<MX_ACT_RELU, OI, WIDE, TB>(a, acc, mw, nw); break;
+    case MX_ACT_SILU: store_results<MX_ACT_SILU, OI, WIDE, TB>(a, acc, mw, nw); break;
+    case MX_ACT_HARDSWISH: store_results<MX_ACT_HARDSWISH, OI, WIDE, TB>(a, acc, mw, nw); break;
+    case MX_ACT_TANH: store_results<MX_ACT_TANH, OI, WIDE, TB>(a, acc, mw, nw); break;
+    default: store_results<MX_ACT_NONE, OI, WIDE, TB>(a, acc, mw, nw); break;
+  }
+}
+
+constexpr size_t kCounterBytes = 64 * 1024;  // of the backend's scratch: arrival counters, zero between launches
+
+template <class Tile, bool WIDE, bool DMA>
+int run_dense_tiles(mx_backend* b, const char* name, DenseArgs a, int slices) {
+  const int64_t tm = ((int64_t)a.M + Tile::kRows - 1) / Tile::kRows, tn = ((int64_t)a.N + Tile::kCols - 1) / Tile::kCols;
+  a.tiles_n = (int)tn;
+  a.kps = std::max((a.KB + slices - 1) / slices, 1);
+  a.S = std::max((a.KB + a.kps - 1) / a.kps, 1);  // K = 0: one slice without a block, act(bias)
+  if (tm * tn * a.S >= (int64_t)1 << 31) return set_error(MX_ERR_INVALID, "F8Dense: more than 2^31 workgroups");
+  if (a.S > 1) {
+    void* scratch = nullptr;
+    MX_TRY(ensure_scratch(b, kCounterBytes + (size_t)(tm * tn * a.S) * Tile::kPartBytes, &scratch));
+    a.arrived = (uint32_t*)scratch;
+    a.part = (char*)scratch + kCounterBytes;
+  }
+  auto k = a.oi ? f8_dense_tiles_kernel<Tile, true, WIDE, DMA> : f8_dense_tiles_kernel<Tile, false, WIDE, DMA>;
+  MX_CHECK_HIP(hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, Tile::kLds));
+  return launch(b, name, [&] { dispatch(k, dim3((unsigned)(tm * tn * a.S)), dim3(Tile::kThreads), Tile::kLds, b->stream, a); });
+}
+
+}  // namespace
+}  // namespace f8
+}  // namespace mx

@@ -167,7 +167,7 @@ __global__ __launch_bounds__(64 * NW) void f8_skinny_kernel(DenseArgs a) {
 //                  [14336] x 4096   18.6  21.0  12.4  12.0               [4096] x 4096           8.5   9.6   7.1   8.2
 //                                                              8 rows    [14336] x 4096         15.1  20.7  14.0  14.2
 // From 768 strips the CUs are full with two operands, which share the lanes' x (as many bytes as the weights with 16
-// rows); from 512 with four waves; below, the waves have to come from K, and their sums cost the rows of codes more.
+// rows); from 512 with four waves; below, the waves have to come from K, and with more rows their sums cost more.
 template <int X, bool WIDE>
 int run_skinny(mx_backend* b, const char* name, const DenseArgs& a) {
   auto go = [&](auto k, int waves, int c) {
@@ -175,11 +175,11 @@ int run_skinny(mx_backend* b, const char* name, const DenseArgs& a) {
     return launch(b, name, [&] { dispatch(k, dim3((unsigned)strips), dim3(64 * waves), 0, b->stream, a); });
   };
   const int strips = (int)(((int64_t)a.N + 15) / 16);
-  if constexpr (X == kCodes) {
+  if (a.M <= kFloatRows) {  // float rows and their codes alike: the same order of sums, the same bits
+    if (strips < 512) return go(f8_skinny_kernel<X, WIDE, 16, 1>, 16, 1);
+  } else if constexpr (X == kCodes) {
     if (strips >= 768) return go(f8_skinny_kernel<X, WIDE, 4, 2>, 4, 2);
     if (strips < 512) return go(f8_skinny_kernel<X, WIDE, 8, 1>, 8, 1);
-  } else {
-    if (strips < 512) return go(f8_skinny_kernel<X, WIDE, 16, 1>, 16, 1);
   }
   return go(f8_skinny_kernel<X, WIDE, 4, 1>, 4, 1);
 }
