@@ -445,14 +445,18 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(Dense
     }
     __syncthreads();
     if (!s_last) return;
-#pragma unroll 1
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int b = 0; b < TB; ++b) acc[c][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kTogether = TB <= 2 ? 4 : 1;  // slices in flight at a time
+#pragma unroll kTogether
     for (int sl = 0; sl < a.S; ++sl)
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int b = 0; b < TB; ++b) {
-          const f32x4 o = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(prs, at(sl, c, b), 0, kSc1));
-          acc[c][b] = sl == 0 ? o : acc[c][b] + o;
+          acc[c][b] += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(prs, at(sl, c, b), 0, kSc1));
         }
   }
   const int mw = m0 + 16 * TB * wm, nw = n0 + 64 * wn;

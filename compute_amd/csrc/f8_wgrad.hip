@@ -25,7 +25,9 @@ struct WGradArgs {
   void* out;
   int M, K, N, KB;
   int out_dt, oi, vec_out;
-  int tiles_n;
+  int tiles_n, slices, tokens;  // slices of the tokens of a tile, tokens of a slice
+  char* part;                   // [tile][slice] sums (slices > 1)
+  uint32_t* arrived;            // [tile], zero between launches
 };
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -48,11 +50,11 @@ __device__ __forceinline__ void parts_of(float v, uint16_t (&p)[3]) {
   p[2] = (uint16_t)(__float_as_uint(r2) >> 16);
 }
 
-// A workgroup computes W (k) x W (n) in WK x WN waves of 32 TK x 32 TN; tokens in steps of S.
+// A workgroup computes kK (k) x kN (n) in WK x WN waves of 32 TK x 32 TN; tokens in steps of S.
 template <int WK_, int WN_, int TK_, int TN_, int S_, int OCC>
 struct Tile {
-  static constexpr int WK = WK_, WN = WN_, TK = TK_, TN = TN_, S = S_, W = 32 * TK * WK, kThreads = 64 * WK * WN, kOccupancy = OCC;
-  static_assert(W == 32 * TN * WN, "square tiles");
+  static constexpr int WK = WK_, WN = WN_, TK = TK_, TN = TN_, S = S_, kThreads = 64 * WK * WN, kOccupancy = OCC;
+  static constexpr int kK = 32 * TK * WK, kN = 32 * TN * WN, kPartBytes = 4 * kK * kN;
 };
 //
 // Staging.  The codes and dy of a step travel through registers, requested a step ahead: 16 codes a chunk,
@@ -91,78 +93,91 @@ struct Window {
 template <class Tile, bool F32, bool OI, bool WHOLE>
 __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_kernel(WGradArgs a) {
   constexpr int TK = Tile::TK, TN = Tile::TN, S = Tile::S, kThreads = Tile::kThreads;
-  constexpr int P = F32 ? 3 : 1, W = Tile::W;          // parts of dy, columns of a tile
-  constexpr int kRow = 2 * W;                          // bytes of a row in LDS
-  constexpr int kBuf = S * kRow;                       // one operand (part) of a step
-  constexpr int kStep = (1 + P) * kBuf;                // LDS of a step
-  constexpr int CX = S * W / 16 / kThreads;            // chunks of x a thread stages
-  constexpr int CD = S * W / 8 / kThreads;             // chunks of dy
-  constexpr int RX = kThreads / (W / 16), RD = kThreads / (W / 8);  // rows between a thread's chunks
+  constexpr int P = F32 ? 3 : 1, WX = Tile::kK, WD = Tile::kN;  // parts of dy, columns of the operands
+  constexpr int kXRow = 2 * WX, kDRow = 2 * WD;        // bytes of a row in LDS
+  constexpr int kXBuf = S * kXRow, kDBuf = S * kDRow;  // x and a part of dy of a step
+  constexpr int kStep = kXBuf + P * kDBuf;             // LDS of a step
+  constexpr int CX = S * WX / 16 / kThreads;           // chunks of x a thread stages
+  constexpr int CD = S * WD / 8 / kThreads;            // chunks of dy
+  constexpr int RX = kThreads / (WX / 16), RD = kThreads / (WD / 8);  // rows between a thread's chunks
   constexpr int kParts = S / 16, kPart = P * TN, G = kParts * kPart;
   constexpr int kRing = 4, kLast = kRing - 1;          // groups after the barrier
-  constexpr int kPieces = 2 * CX + CD;                 // staged at a time: half a chunk of x or one of dy
+  constexpr int kPieces = 2 * CX + CD;                 // staged at a time: half a chunk of x or one of dy, mixed evenly
+  auto x_before = [](int p) constexpr { return (p * 2 * CX + kPieces - 1) / kPieces; };  // pieces of x among the first p
   constexpr int kStageGroups = G - kLast < kPieces ? G - kLast : kPieces, kStageFrom = G - kLast - kStageGroups;
-  static_assert(2 * CX == CD, "pieces alternate between x and dy");
   constexpr int kPerGroup = (kPieces + kStageGroups - 1) / kStageGroups;
   constexpr int H = F32 ? 2 : 1, E = F32 ? 4 : 2;      // loads of a dy chunk, bytes of a value
-  static_assert(CX * 16 * kThreads == S * W && CD * 8 * kThreads == S * W, "whole chunks");
+  static_assert(CX * 16 * kThreads == S * WX && CD * 8 * kThreads == S * WD, "whole chunks");
   static_assert(kParts % 2 == 0 && kPart >= TK, "the sets of x operands alternate, and one is read while the other is used");
   static_assert(G % kRing == 0, "the ring's slots are the same in every step");
-  static_assert((kStep & (kStep - 1)) == 0, "the buffers alternate by an XOR");
+  static_assert(kStep % 1024 == 0, "the buffers differ above the bits of a piece");
   static_assert((TK & (TK - 1)) == 0 && (TN & (TN - 1)) == 0, "a wave's pieces start on a multiple of their number: an XOR picks one");
-  extern __shared__ __align__(1024) uint8_t lds[];     // [2][1 + P][S][W] bf16
+  extern __shared__ __align__(1024) uint8_t lds[];     // [2]: x [S][WX], then the parts of dy [P][S][WD], bf16
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, i = lane % 32, g = lane / 32;
-  const int tiles_k = (a.K + W - 1) / W;
-  int kt, nt;
+  int kt, nt, tile, slice;
   {
-    // Runs of 4 tiles of k by all tiles of n: a run's workgroups share their rows of x and dy in an L2.
-    const int t = xcd_order((int)blockIdx.x, (int)gridDim.x);
+    // Runs of 4 tiles of k by all tiles of n: a run's workgroups share their rows of x and dy in an L2.  A tile's
+    // slices of the tokens are neighbours.
+    const int it = xcd_order((int)blockIdx.x, (int)gridDim.x), t = it / a.slices;
+    tile = t;
+    slice = it - t * a.slices;
+    const int tiles_k = (int)gridDim.x / a.slices / a.tiles_n;
     const int per = 4 * a.tiles_n, q = t / per, rows = min(4, tiles_k - 4 * q), in = t - q * per;
     kt = 4 * q + in % rows;
     nt = in / rows;
   }
-  const int k0 = kt * W, n0 = nt * W;
+  const int k0 = kt * WX, n0 = nt * WD;
+  const int from = slice * a.tokens, to = min(a.M, from + a.tokens);  // the slice's tokens
   const int64_t x_total = (int64_t)a.M * a.K, dy_total = (int64_t)a.M * a.N;
-  const int xrow = tid / (W / 16), xk = k0 + 16 * (tid % (W / 16));  // the thread's first chunk of a step
-  const int drow = tid / (W / 8), dn = n0 + 8 * (tid % (W / 8));
+  const int xrow = tid / (WX / 16), xk = k0 + 16 * (tid % (WX / 16));  // the thread's first chunk of a step
+  const int drow = tid / (WD / 8), dn = n0 + 8 * (tid % (WD / 8));
   const int kb = min(xk / kBlock, a.KB - 1);
 
   u32x4 xr[CX], dr[CD][H];
   float sr[CX];
-  // WHOLE: byte offsets of the thread's chunks within a step (below 64 rows of 2^26 bytes), and the
-  // windows of the step requested next.
+  // Byte offsets of the thread's chunks within a step (below 64 rows of 2^26 bytes), and the windows of the
+  // step requested next.
   uint32_t x_off[CX], s_off[CX], d_off[CD];
 #pragma unroll
   for (int j = 0; j < CX; ++j) {
-    x_off[j] = (uint32_t)(xrow + j * RX) * (uint32_t)a.K + (uint32_t)min(xk, a.K - 16);
+    x_off[j] = (uint32_t)(xrow + j * RX) * (uint32_t)a.K + (uint32_t)min(xk, a.K - (WHOLE ? 16 : 1));
     s_off[j] = 4 * ((uint32_t)(xrow + j * RX) * (uint32_t)a.KB + (uint32_t)kb);
   }
 #pragma unroll
-  for (int j = 0; j < CD; ++j) d_off[j] = E * ((uint32_t)(drow + j * RD) * (uint32_t)a.N + (uint32_t)min(dn, a.N - 8));
-  Window xw{a.x, x_total}, sw{(const uint8_t*)a.x_scale, (int64_t)a.M * a.KB * 4}, dw{(const uint8_t*)a.dy, dy_total * E};
+  for (int j = 0; j < CD; ++j) d_off[j] = E * ((uint32_t)(drow + j * RD) * (uint32_t)a.N + (uint32_t)min(dn, a.N - (WHOLE ? 8 : 1)));
+  // (A slice's windows end with its tokens.)
+  Window xw{a.x + (int64_t)from * a.K, (int64_t)(to - from) * a.K};
+  Window sw{(const uint8_t*)(a.x_scale + (int64_t)from * a.KB), (int64_t)(to - from) * a.KB * 4};
+  Window dw{(const uint8_t*)a.dy + (int64_t)from * a.N * E, (int64_t)(to - from) * a.N * E};
   auto advance = [&]() __attribute__((always_inline)) {
     xw.move((int64_t)S * a.K);
     sw.move((int64_t)S * a.KB * 4);
     dw.move((int64_t)S * a.N * E);
   };
-  auto request = [&](int m0, int piece) __attribute__((always_inline)) {
-    if (piece % 2 == 0) {
-      const int j = piece / 4;
-      if (piece % 4 == 0) return;  // the first half of a chunk: the second still stands in the registers
+  auto request = [&](auto inside, int m0, int piece) __attribute__((always_inline)) {
+    constexpr bool kInside = decltype(inside)::value;
+    if (x_before(piece + 1) > x_before(piece)) {
+      const int j = x_before(piece) / 2;
+      if (x_before(piece) % 2 == 0) return;  // the first half of a chunk: the second still stands in the registers
       if constexpr (WHOLE) {
         xr[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(xw.resource(), x_off[j], 0, 0));
         sr[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(sw.resource(), s_off[j], 0, 0));
+      } else if constexpr (kInside) {
+        xr[j] = load16_any(xw.p + x_off[j]);
+        sr[j] = *(const float*)(sw.p + s_off[j]);
       } else {
         const int64_t row = min(m0 + xrow + j * RX, a.M - 1), at = row * a.K + min(xk, a.K - 1);
         xr[j] = load16(a.x + at, x_total - at);
         sr[j] = a.x_scale[row * a.KB + kb];
       }
     } else {
-      const int j = piece / 2;
+      const int j = piece - x_before(piece);
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         if constexpr (WHOLE) {
           dr[j][h] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(dw.resource(), d_off[j], 16 * h, 0));
+        } else if constexpr (kInside) {
+          dr[j][h] = load16_any(dw.p + d_off[j] + 16 * h);
         } else {
           const int64_t at = (int64_t)min(m0 + drow + j * RD, a.M - 1) * a.N + min(dn, a.N - 1) + 4 * h;
           dr[j][h] = load16((const uint8_t*)a.dy + E * at, E * (dy_total - at));
@@ -171,12 +186,13 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_ker
     }
   };
   // Piece of the step from m0 into LDS at `step`.
-  auto swizzled = [](int m, int piece) { return m * kRow + 32 * (piece ^ (2 * (m & 3))); };
-  auto stage = [&](int m0, uint32_t step, int piece) __attribute__((always_inline)) {
+  auto swizzled = [](int row, int m, int piece) { return m * row + 32 * (piece ^ (2 * (m & 3))); };
+  auto stage = [&](auto inside, int m0, uint32_t step, int piece) __attribute__((always_inline)) {
+    constexpr bool kMask = !WHOLE && !decltype(inside)::value;
     uint8_t* xb = lds + step;
-    if (piece % 2 == 0) {
-      const int j = piece / 4, half = piece / 2 % 2;
-      if (!WHOLE && half == 0 && m0 + xrow + j * RX >= a.M) xr[j] = u32x4{0u, 0u, 0u, 0u};
+    if (x_before(piece + 1) > x_before(piece)) {
+      const int j = x_before(piece) / 2, half = x_before(piece) % 2;
+      if (kMask && half == 0 && m0 + xrow + j * RX >= to) xr[j] = u32x4{0u, 0u, 0u, 0u};
       u32x4 o;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
@@ -186,13 +202,13 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_ker
         o[2 * w] = __builtin_bit_cast(uint32_t, __builtin_convertvector(lo, bf16x2));
         o[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(hi, bf16x2));
       }
-      *(u32x4*)(xb + swizzled(xrow + j * RX, tid % (W / 16)) + 16 * half) = o;
+      *(u32x4*)(xb + swizzled(kXRow, xrow + j * RX, tid % (WX / 16)) + 16 * half) = o;
     } else {
-      const int j = piece / 2, c = tid % (W / 8);
+      const int j = piece - x_before(piece), c = tid % (WD / 8);
 #pragma unroll
       for (int h = 0; h < H; ++h)
-        if (!WHOLE && m0 + drow + j * RD >= a.M) dr[j][h] = u32x4{0u, 0u, 0u, 0u};
-      uint8_t* q = xb + kBuf + swizzled(drow + j * RD, c / 2) + 16 * (c % 2);
+        if (kMask && m0 + drow + j * RD >= to) dr[j][h] = u32x4{0u, 0u, 0u, 0u};
+      uint8_t* q = xb + kXBuf + swizzled(kDRow, drow + j * RD, c / 2) + 16 * (c % 2);
       if constexpr (F32) {
         uint16_t p[8][3];
 #pragma unroll
@@ -202,7 +218,7 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_ker
           u32x4 o;
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] = (uint32_t)p[2 * e][t] | (uint32_t)p[2 * e + 1][t] << 16;
-          *(u32x4*)(q + t * kBuf) = o;
+          *(u32x4*)(q + t * kDBuf) = o;
         }
       } else {
         *(u32x4*)q = dr[j][0];
@@ -213,40 +229,28 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_ker
   // Operand reads: token 8 g + 4 h + (lane % 16) / 4 of 16, columns 32 t + 16 (i / 16) + 4 (lane % 4) ..
   const int wk = wave / Tile::WN, wn = wave % Tile::WN;
   const uint32_t base = lds_addr(lds);
-  auto read_base = [&](int piece) { return base + (uint32_t)swizzled(8 * g + lane % 16 / 4, piece + i / 16) + 8 * (lane % 4); };
-  const uint32_t xa = read_base(2 * wk * TK), da = read_base(2 * wn * TN) + kBuf;
-  auto operand = [&](uint32_t at, int t, int off) __attribute__((always_inline)) {
+  auto read_base = [&](int row, int piece) { return base + (uint32_t)swizzled(row, 8 * g + lane % 16 / 4, piece + i / 16) + 8 * (lane % 4); };
+  const uint32_t xa = read_base(kXRow, 2 * wk * TK), da = read_base(kDRow, 2 * wn * TN) + kXBuf;
+  auto operand = [&](uint32_t at, int row, int t, int off) __attribute__((always_inline)) {
     const uint32_t p = (at ^ (uint32_t)(64 * t)) + (uint32_t)off;
-    const u32x2 lo = read_tr16(p), hi = read_tr16(p + 4 * kRow);
+    const u32x2 lo = read_tr16(p), hi = read_tr16(p + 4 * row);
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
   u32x4 xo[2][TK], dv[kRing];
   auto read_x = [&](int set, int t, uint32_t step, int part) __attribute__((always_inline)) {
-    xo[set][t] = operand(xa + step, t, part * 16 * kRow);
+    xo[set][t] = operand(xa + step, kXRow, t, part * 16 * kXRow);
   };
   auto read_dy = [&](int q, uint32_t step) __attribute__((always_inline)) {  // of group q of a step
-    dv[q % kRing] = operand(da + step, q % TN, (q / TN % P) * kBuf + q / (TN * P) * 16 * kRow);
+    dv[q % kRing] = operand(da + step, kDRow, q % TN, (q / TN % P) * kDBuf + q / (TN * P) * 16 * kDRow);
   };
 
   f32x16 acc[TK][TN] = {};
-  if (a.M > 0) {
-#pragma unroll
-    for (int p = 0; p < kPieces; ++p) request(0, p);
-    if constexpr (WHOLE) advance();
-#pragma unroll
-    for (int p = 0; p < kPieces; ++p) {
-      stage(0, 0, p);
-      request(S, p);
-    }
-    lds_barrier();
-#pragma unroll
-    for (int t = 0; t < TK; ++t) read_x(0, t, 0, 0);
-#pragma unroll
-    for (int q = 0; q < kLast; ++q) read_dy(q, 0);
-    uint32_t cur = 0;
-    for (int m0 = 0; m0 < a.M; m0 += S) {
-      const uint32_t next = cur ^ kStep;
-      if constexpr (WHOLE) advance();
+  uint32_t cur = 0;
+  // The step from token m0.  inside (WHOLE: always): what it stages lies before `to` and what it requests in the array,
+  // a chunk past a row's end included.
+  auto step = [&](auto inside, int m0) __attribute__((always_inline)) {
+      const uint32_t next = kStep - cur;
+      advance();
 #pragma unroll
       for (int q = 0; q < G; ++q) {
         const int part = q / kPart, set = part % 2;
@@ -271,8 +275,8 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_ker
           for (int e = 0; e < kPerGroup; ++e) {
             const int p = (q - kStageFrom) * kPerGroup + e;
             if (p < kPieces) {
-              stage(m0 + S, next, p);
-              request(m0 + 2 * S, p);
+              stage(inside, m0 + S, next, p);
+              request(inside, m0 + 2 * S, p);
             }
           }
         }
@@ -283,7 +287,7 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_ker
           else
             acc[t][q % TN] = mfma_bf16(dv[q % kRing], xo[set][t], acc[t][q % TN]);
         }
-        if constexpr (WHOLE) {
+        if constexpr (WHOLE || decltype(inside)::value) {
 #pragma unroll
           for (int t = 0; t < TK; ++t) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
@@ -295,7 +299,76 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_ker
         }
       }
       cur = next;
+  };
+  if (from < to) {
+    constexpr std::integral_constant<bool, WHOLE> edge{};
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) request(edge, from, p);
+    advance();
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      stage(edge, from, 0, p);
+      request(edge, from + S, p);
     }
+    lds_barrier();
+#pragma unroll
+    for (int t = 0; t < TK; ++t) read_x(0, t, 0, 0);
+#pragma unroll
+    for (int q = 0; q < kLast; ++q) read_dy(q, 0);
+    int m0 = from;
+    if constexpr (!WHOLE) {
+      const int64_t most = min(a.K, a.N);
+      if (a.K <= 1 << 24 && a.N <= 1 << 24)
+        for (; m0 + 3 * S <= to && (int64_t)(a.M - (m0 + 3 * S)) * most >= 16; m0 += S) step(std::true_type{}, m0);
+    }
+    for (; m0 < to; m0 += S) step(edge, m0);
+  }
+
+  if (a.slices > 1) {
+    // The slices' sums meet in scratch, stored and loaded with the agent-scope coherence bit (sc1): the slices may run
+    // on different XCDs.  The last to arrive adds them in order and goes on; it leaves the counter at zero.
+    __shared__ int s_last;
+    constexpr int kSc1 = 16;
+    const __amdgpu_buffer_rsrc_t prs = __builtin_amdgcn_make_buffer_rsrc((char*)a.part + (int64_t)tile * a.slices * Tile::kPartBytes, 0,
+                                                                         a.slices * Tile::kPartBytes, 0x00027000);
+    auto at = [&](int sl, int t, int n, int q) {
+      return (uint32_t)(sl * Tile::kPartBytes + (((t * TN + n) * 4 + q) * kThreads + tid) * 16);
+    };
+#pragma unroll
+    for (int t = 0; t < TK; ++t)
+#pragma unroll
+      for (int n = 0; n < TN; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 v = {acc[t][n][4 * q], acc[t][n][4 * q + 1], acc[t][n][4 * q + 2], acc[t][n][4 * q + 3]};
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), prs, at(slice, t, n, q), 0, kSc1);
+        }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) {
+      const uint32_t before = __hip_atomic_fetch_add(&a.arrived[tile], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_last = before + 1u == (uint32_t)a.slices;
+      if (s_last) __hip_atomic_store(&a.arrived[tile], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!s_last) return;
+#pragma unroll
+    for (int t = 0; t < TK; ++t)
+#pragma unroll
+      for (int n = 0; n < TN; ++n) acc[t][n] = f32x16{};
+    constexpr int kTogether = TK * TN <= 4 ? 2 : 1;  // slices in flight at a time
+#pragma unroll kTogether
+    for (int sl = 0; sl < a.slices; ++sl)
+#pragma unroll
+      for (int t = 0; t < TK; ++t)
+#pragma unroll
+        for (int n = 0; n < TN; ++n)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(prs, at(sl, t, n, q), 0, kSc1));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[t][n][4 * q + r] += v[r];
+          }
   }
 
   // Result (t, n): of its 32 x 32 the lane holds column i and rows 8 q + 4 g .. + 3.  The operand whose
@@ -316,47 +389,83 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_ker
     }
 }
 
+constexpr size_t kCounterBytes = 64 * 1024;  // of the backend's scratch: arrival counters, zero between launches
+
 template <class Tile, bool F32>
-int run_tiles(mx_backend* b, const char* name, WGradArgs a, bool whole) {
-  constexpr int W = Tile::W, P = F32 ? 3 : 1, kLds = 2 * (1 + P) * Tile::S * W * 2;
-  const int64_t tk = (a.K + W - 1) / W, tn = (a.N + W - 1) / W;
-  if (tk * tn >= (int64_t)1 << 31) return set_error(MX_ERR_INVALID, "F8WeightGradient: more than 2^31 workgroups");
+int run_tiles(mx_backend* b, const char* name, WGradArgs a, bool whole, int slices) {
+  constexpr int P = F32 ? 3 : 1, kLds = 2 * 2 * Tile::S * (Tile::kK + P * Tile::kN);
+  const int64_t tk = (a.K + Tile::kK - 1) / Tile::kK, tn = (a.N + Tile::kN - 1) / Tile::kN;
+  const int steps = (a.M + Tile::S - 1) / Tile::S, per = (steps + slices - 1) / slices;
+  a.tokens = std::max(per, 1) * Tile::S;
+  a.slices = std::max((a.M + a.tokens - 1) / a.tokens, 1);
   a.tiles_n = (int)tn;
+  if (tk * tn * a.slices >= (int64_t)1 << 31) return set_error(MX_ERR_INVALID, "F8WeightGradient: more than 2^31 workgroups");
+  if (a.slices > 1) {
+    void* scratch = nullptr;
+    MX_TRY(ensure_scratch(b, kCounterBytes + (size_t)(tk * tn * a.slices) * Tile::kPartBytes, &scratch));
+    a.arrived = (uint32_t*)scratch;
+    a.part = (char*)scratch + kCounterBytes;
+  }
   auto k = a.oi ? (whole ? f8_wgrad_kernel<Tile, F32, true, true> : f8_wgrad_kernel<Tile, F32, true, false>)
                 : (whole ? f8_wgrad_kernel<Tile, F32, false, true> : f8_wgrad_kernel<Tile, F32, false, false>);
   MX_CHECK_HIP(hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
-  return launch(b, name, [&] { dispatch(k, dim3((unsigned)(tk * tn)), dim3(Tile::kThreads), kLds, b->stream, a); });
+  return launch(b, name, [&] { dispatch(k, dim3((unsigned)(tk * tn * a.slices)), dim3(Tile::kThreads), kLds, b->stream, a); });
 }
 
-enum class Plan { kF32, kBf16, kBf16Large };
+using Tile256 = Tile<4, 2, 2, 4, 64, 2>;
+using Tile128 = Tile<2, 2, 2, 2, 64, 2>;
+using TileF32 = Tile<2, 2, 2, 2, 32, 2>;
 
-Plan plan_of(const F8WGradDesc& d) {
-  if (d.dy_dt == MX_DTYPE_FLOAT32) return Plan::kF32;
-  const int64_t tiles = ((d.K + 255) / 256) * ((d.N + 255) / 256);
-  return tiles >= 192 ? Plan::kBf16Large : Plan::kBf16;
+struct Choice {
+  bool large;  // 256 x 256 tiles
+  int slices;
+};
+
+// The tile and the number of token slices that take the least time by the measured times of their parts: a launch 3 us; a
+// round of workgroups its first loads and its stores, and its steps (the 128 x 128 tiles run two to a CU); for sums that
+// meet in scratch 3 us and 1.2 a slice.  Measured (us; 256 x 256 | 128 x 128 by slices 1, 2, 3, 4, 6, 8):
+//   bf16  2048 x 4096 x 14336    265 | 346         4096 x 1024 x 1024    -  | 47 33 28 26 31 33
+//         2048 x 4096 x 4096      69 |  87          333 x 1536 x 384     -  | 9.7 12 12 12 16 16
+//         2048 x 2048 x 2048      -  |  31 34 42
+//   f32    333 x 1536 x 384       18.0 16.5 15.6 16.2 18.0 17.9    4000 x 512 x 512     148 79 57 47 38 35 (34 in 12)
+//         2048 x 2048 x 2048      85.8 75.6 82.8
+// Tiles of 128 x 256 and 256 x 128, two workgroups a CU, took 291 and 294 us for the first.
+Choice plan_of(const F8WGradDesc& d) {
+  const bool f32 = d.dy_dt == MX_DTYPE_FLOAT32;
+  Choice best{false, 1};
+  double least = 1e30;
+  for (int large = 0; large < (f32 ? 1 : 2); ++large) {
+    const int side = large ? 256 : 128, S = f32 ? 32 : 64, slots = large ? 256 : 512;
+    const int64_t tiles = ((d.K + side - 1) / side) * ((d.N + side - 1) / side), steps = (d.M + S - 1) / S;
+    for (int slices = 1; slices <= 16 && slices <= std::max<int64_t>(steps, 1); ++slices) {
+      const int64_t per = (steps + slices - 1) / slices;
+      const double part = (double)tiles * slices * side * side * 4;
+      if (slices > 1 && ((steps + per - 1) / per != slices || tiles > (int64_t)(kCounterBytes / 4) || part > 64e6)) continue;
+      const bool alone = tiles * slices <= 256;  // at most one workgroup a CU
+      const double step = large ? 1.72 : f32 ? (alone ? 1.28 : 1.9) : alone ? 0.83 : 1.2;
+      const double us = 3 + (double)((tiles * slices + slots - 1) / slots) * ((large ? 11 : alone ? 2 : 5) + (double)per * step) + (slices > 1 ? 3 + 1.2 * slices : 0);
+      if (us < least) {
+        least = us;
+        best = {large != 0, slices};
+      }
+    }
+  }
+  return best;
 }
 
 }  // namespace
 
-const char* f8_wgrad_name(const F8WGradDesc& d) {
-  switch (plan_of(d)) {
-    case Plan::kF32: return "f8_wgrad_f32_128";
-    case Plan::kBf16: return "f8_wgrad_bf16_128";
-    default: return "f8_wgrad_bf16_256";
-  }
-}
+const char* f8_wgrad_name(const F8WGradDesc& d) { return d.dy_dt == MX_DTYPE_FLOAT32 ? "f8_wgrad_f32" : "f8_wgrad_bf16"; }
 
 int f8_wgrad_run(mx_backend* b, const F8WGradDesc& d) {
   if (d.K == 0 || d.N == 0) return MX_OK;
-  const WGradArgs a{d.x, d.x_scale, d.dy, d.out, (int)d.M, (int)d.K, (int)d.N, (int)blocks(d.K), d.out_dt, d.oi,
-                    (d.oi ? d.K : d.N) % 4 == 0 && ((uintptr_t)d.out & (d.out_dt == MX_DTYPE_FLOAT32 ? 15 : 7)) == 0, 0};
+  const bool vec = (d.oi ? d.K : d.N) % 4 == 0 && ((uintptr_t)d.out & (d.out_dt == MX_DTYPE_FLOAT32 ? 15 : 7)) == 0;
+  const WGradArgs a{d.x, d.x_scale, d.dy, d.out, (int)d.M, (int)d.K, (int)d.N, (int)blocks(d.K), d.out_dt, d.oi, vec, 0, 1, 0, nullptr, nullptr};
   const bool whole = d.K % 16 == 0 && d.N % 8 == 0 && d.K <= 1 << 24 && d.N <= 1 << 24 && aligned16(d.x) && aligned16(d.dy);
   const char* name = f8_wgrad_name(d);
-  switch (plan_of(d)) {
-    case Plan::kF32: return run_tiles<Tile<2, 2, 2, 2, 32, 2>, true>(b, name, a, whole);
-    case Plan::kBf16: return run_tiles<Tile<2, 2, 2, 2, 64, 2>, false>(b, name, a, whole);
-    default: return run_tiles<Tile<4, 2, 2, 4, 64, 2>, false>(b, name, a, whole);
-  }
+  const Choice c = plan_of(d);
+  if (d.dy_dt == MX_DTYPE_FLOAT32) return run_tiles<TileF32, true>(b, name, a, whole, c.slices);
+  return c.large ? run_tiles<Tile256, false>(b, name, a, whole, c.slices) : run_tiles<Tile128, false>(b, name, a, whole, c.slices);
 }
 
 }  // namespace mx
