@@ -66,23 +66,29 @@ __device__ __forceinline__ u32x4 load16(const uint8_t* p, int64_t n) {
   return v;
 }
 
-// Four consecutive results from element `at`, of which the first n are in the row; vec: four are whole
-// and aligned.
+// Four consecutive results from element `at`, of which the first n are in the row; vec: they are whole and aligned.
+// (Unaligned ones still go as one store: value by value an instruction writes 4 bytes to each of 64 places.)
 __device__ __forceinline__ void store4(void* out, int64_t at, int n, bool vec, int dt, const f32x4& v) {
-  if (vec) {
-    if (n <= 0) return;
+  if (vec ? n > 0 : n >= 4) {
     if (dt == MX_DTYPE_FLOAT32) {
-      *(f32x4*)((float*)out + at) = v;
+      if (vec)
+        *(f32x4*)((float*)out + at) = v;
+      else
+        __builtin_memcpy((float*)out + at, &v, 16);
     } else {
       const f32x2 lo = {v[0], v[1]}, hi = {v[2], v[3]};
-      *(u32x2*)((uint16_t*)out + at) = u32x2{__builtin_bit_cast(uint32_t, __builtin_convertvector(lo, bf16x2)),
-                                             __builtin_bit_cast(uint32_t, __builtin_convertvector(hi, bf16x2))};
+      const u32x2 o = {__builtin_bit_cast(uint32_t, __builtin_convertvector(lo, bf16x2)),
+                       __builtin_bit_cast(uint32_t, __builtin_convertvector(hi, bf16x2))};
+      if (vec)
+        *(u32x2*)((uint16_t*)out + at) = o;
+      else
+        __builtin_memcpy((uint16_t*)out + at, &o, 8);
     }
-    return;
-  }
+  } else if (!vec) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (r < n) store_f(out, at + r, dt, v[r]);
+    for (int r = 0; r < 3; ++r)
+      if (r < n) store_f(out, at + r, dt, v[r]);
+  }
 }
 
 // Workgroup barrier ordering LDS only: global loads in flight stay in flight.

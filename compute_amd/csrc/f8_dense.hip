@@ -7,8 +7,8 @@ namespace {
 using namespace f8;
 
 using Tile256x256 = DenseTile<4, 2, 8, 2>;  // columns x rows
-using Tile256x128 = DenseTile<4, 2, 4, 2>;
-using Tile128x128 = DenseTile<2, 4, 2, 3>;
+using Tile256x128 = DenseTile<4, 2, 4, 3>;
+using Tile128x128 = DenseTile<2, 4, 2, 3>;  // (one more buffer makes the smaller tiles slower by up to 5%)
 using Tile128x64 = DenseTile<2, 2, 2, 4>;
 using Tile64x128 = DenseTile<1, 4, 2, 4>;
 using Tile64x64 = DenseTile<1, 2, 2, 4>;
@@ -20,22 +20,29 @@ struct DenseChoice {
 };
 
 // The tile and the number of K slices that take the least time by the measured times of their parts: a launch 3 us; a
-// round of workgroups its first loads and its stores 4.5 us, and a step of 128 k (below, us, with every CU at work); 2 us
-// for sums that meet in scratch and their bytes, out and back, at 14 TB/s (they mostly stay in the caches).  Against
-// sweeps of all of them at 17 shapes the choice is the best or within 8% of it, for instance (us, columns x rows, slices)
-//   [97,4096] x 14336    64x128 20.9, 128x128 in two 21.0, 256x128 in three 25.2, 64x64 25.0
-//   [256,4096] x 4096    128x64 in two 16.2, 128x128 in four 17.3, 64x128 20.4
-//   [512,4096] x 11008   256x128 45.9, 256x256 in two 56.3, 128x128 61.5
-//   [2048,4096] x 4096   256x128 44.8, 128x128 55.8, 256x256 in two 60.7
+// round of workgroups its first loads and its stores 4.5 us, and a step of 128 k (below, us, with every CU at work); for sums
+// that meet in scratch 1.2 us, 0.3 us a slice and their bytes, out and back, at 14 TB/s (they mostly stay in the
+// caches).  Against sweeps of all of them at 20 shapes the choice is within 8% of the best, once 15% off, for instance (us, columns x rows,
+// slices, bfloat16 results)
+//   [97,4096] x 14336     128x128 in two 21.1, 64x128 21.9, 128x64 22.3, 256x128 in three 24.8
+//   [256,4096] x 4096     128x64 in two 16.5, 64x128 in two 16.7, 128x128 in three 17.3
+//   [512,4096] x 11008    256x128 42.2, 256x256 in two 51.9, 128x128 58.4
+//   [2048,4096] x 4096    256x128 42.6, 128x128 59.6, 256x256 60.5
+//   [4096,4096] x 4096    256x256 68.5 (2.0 PFLOP/s), 256x128 83.7, 128x128 116
+//   [2048,4096] x 14336   256x256 134, 256x128 167, 128x128 212
 struct TileCost {
   int cols, rows, slots;  // workgroups at once on 256 CUs
   float step, wide_step;  // (float32 results)
   float alone, wide_alone;  // with at most one workgroup a CU
   bool staged;              // also built for chunks through registers
 };
-constexpr TileCost kTileCosts[] = {{256, 256, 256, 1.83f, 1e9f, 1.83f, 1e9f, false}, {256, 128, 256, 1.2f, 2.35f, 1.2f, 2.35f, false},
-                                   {128, 128, 256, 0.72f, 1.32f, 0.72f, 1.32f, true}, {128, 64, 256, 0.43f, 0.78f, 0.43f, 0.78f, true},
-                                   {64, 128, 256, 0.43f, 0.78f, 0.43f, 0.78f, false}, {64, 64, 512, 0.55f, 0.95f, 0.33f, 0.55f, true}};
+constexpr float kNever = 1e9f;  // not built: bfloat16 operands of eight groups have no registers
+constexpr TileCost kTileCosts[] = {{256, 256, 256, 1.96f, kNever, 1.96f, kNever, false},
+                                   {256, 128, 256, 1.13f, 2.05f, 1.13f, 2.05f, false},
+                                   {128, 128, 256, 0.73f, 1.34f, 0.58f, 1.15f, true},
+                                   {128, 64, 256, 0.50f, 0.82f, 0.44f, 0.76f, true},
+                                   {64, 128, 256, 0.50f, 0.82f, 0.43f, 0.74f, false},
+                                   {64, 64, 512, 0.65f, 1.05f, 0.40f, 0.68f, true}};
 
 DenseChoice dense_plan(const F8DenseDesc& d) {
   if (skinny_fits(d)) return {DensePlan::kSkinny, 0, 1};
@@ -56,7 +63,7 @@ DenseChoice dense_plan(const F8DenseDesc& d) {
       if (S > 1 && (used != S || tiles > (int64_t)(kCounterBytes / 4) || part > 64e6)) continue;
       const bool alone = tiles * S <= 256;
       const double step = wide ? (alone ? c.wide_alone : c.wide_step) : alone ? c.alone : c.step;
-      const double us = 3 + (double)((tiles * S + c.slots - 1) / c.slots) * (4.5 + (double)per * step) + (S > 1 ? 2 + 2 * part / 14e6 : 0);
+      const double us = 3 + (double)((tiles * S + c.slots - 1) / c.slots) * (4.5 + (double)per * step) + (S > 1 ? 1.2 + 0.3 * S + 2 * part / 14e6 : 0);
       if (us < least) {
         least = us;
         best.tile = t;

@@ -37,18 +37,25 @@ namespace {
 // steps ahead, into BUF buffers.  The resources end with their arrays, and past the end LDS gets zeros: rows past M or N and,
 // for w [K, N], rows past K need nothing more.  The last block's chunks past K are sent past the end by their offset.
 //   x, and w [N, K] (OI): rows of 128 bytes.  A lane reads its 32 codes as two 16-byte chunks; chunk c of row r lies at
-//     c ^ (r >> 1 & 7) for x, whose operands are 16 consecutive rows, and at c ^ ((r >> 1 & 1) | (r >> 4 & 3) << 1) for
-//     w: operand a of a wave is the rows 16 (i / 4) + 4 a + i % 4 of its 64, which leaves a lane with 16 consecutive
-//     columns over its four operands.  Either way 16 lanes meet every bank once.
+//     c ^ spread(p) with p = r >> 1 & 7 for x, whose operands are 16 consecutive rows, and p = (r >> 1 & 1) | (r >> 4 & 3)
+//     << 1 for w: operand a of a wave is the rows 16 (i / 4) + 4 a + i % 4 of its 64, which leaves a lane with 16
+//     consecutive columns over its four operands.  A 16-byte read takes the lanes 0-3, 12-15, 20-23 and 24-27 at a time,
+//     then 4-11 with 16-19 and 28-31, and so on: pairs of rows 0, 1, 6, 7 of one g with 2 to 5 of its neighbour, whose
+//     chunk differs by 2.  spread() gives the two sets disjoint halves that stay their own under ^ 2, so that they meet
+//     every bank once: 221 bytes a clock, and 118 with c ^ p.
 //   DMA: these loads take whole aligned chunks and 32-bit offsets.  Otherwise the chunks come through registers, from
 //     any address, requested a step ahead and written to the same places of two buffers.
 //   w [K, N] (!OI): 128 rows of k, 64 WN columns, read through the transposing read, eight k at a time; 16-byte chunk c
 //     of row k lies at c ^ k_swizzle(k), which sends the 8 rows and two halves of 16 lanes to all banks.
 //
-// Schedule.  A step is TB groups of four MFMAs, one operand of x against the wave's four of w.  An operand of x is
-// read kRing - 1 groups ahead; a group's sums enter the total during the next group.  The step's barrier stands before
-// its last kRing - 1 groups, whose operands are in registers: behind it the step BUF ahead is requested into the
-// buffer just left, and w's operands are read again as the last group leaves them.
+// Schedule.  A step is TB groups of four MFMAs, one operand of x against the wave's four of w.  Operands of x are read two
+// groups ahead; a group's sums enter the total during the next group.  The step's barrier stands before its last two
+// groups, whose operands are in registers: behind it begin the requests of the step BUF ahead, into the buffer just left, and
+// under those groups travel the first operands of the next step, all of w's among them (in registers of their own, from
+// which a step's start takes them; eight groups have too few registers left and read w's into place after their last use).
+// The requests are spread over the half-groups of a whole step: a wave stands still until its load is taken, 16 cycles each,
+// and 48 KB requested at once by all waves kept the MFMAs waiting for 780 cycles of a step of 2500 (1.04 us a step of 256 x 128 on one
+// CU, 0.85 when spread; the loads alone run at 152 GB/s a CU).
 struct Resource {
   i32x4 d;
 };
@@ -100,6 +107,9 @@ __device__ __forceinline__ u32x4 first_bytes(u32x4 v, int n) {
   }
   return v;
 }
+
+// 0, 1, 6, 7 to 4 .. 7 and 2 .. 5 to 0 .. 3.
+__device__ __forceinline__ int spread(int p) { return (p & 3) | (~(p >> 2 ^ p >> 1) & 1) << 2; }
 
 template <int WN_, int WM_, int TB_, int BUF_>
 struct DenseTile {
@@ -188,9 +198,10 @@ __device__ __forceinline__ f32x4 block_sum(const Operand<true>& a, const Operand
 template <class Tile, bool OI, bool WIDE, bool DMA>
 __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(DenseArgs a) {
   constexpr int TB = Tile::TB, kWaves = Tile::kWaves;
-  constexpr int kRing = 2, kLast = kRing - 1;
+  constexpr int kLast = 2;  // groups behind the barrier
+  constexpr bool kAhead = TB <= 4;  // w's next operands travel into registers of their own
   constexpr int XL = Tile::kXBytes / (1024 * kWaves), WL = Tile::kWBytes / (1024 * kWaves);  // loads a wave a step
-  static_assert(TB % kRing == 0, "the ring's slots are the same in every step");
+  static_assert(TB >= kLast && TB % 2 == 0, "the operands behind the barrier have registers of their own; sums alternate");
   extern __shared__ __align__(1024) uint8_t lds[];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), i = lane % 16, g = lane / 16;
   const uint32_t base = lds_addr(lds);
@@ -214,7 +225,7 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(Dense
   const int last = a.K - (a.KB - 1) * kBlock;  // codes of the last block
 #pragma unroll
   for (int j = 0; j < XL; ++j) {
-    const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ (r >> 1 & 7);
+    const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ spread(r >> 1 & 7);
     x_off[j] = (uint32_t)r * (uint32_t)a.K + 16 * c;
     x_tail[j] = 16 * c >= last ? kPastEnd : 0u;
   }
@@ -222,7 +233,7 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(Dense
 #pragma unroll
   for (int j = 0; j < WL; ++j) {
     if constexpr (OI) {
-      const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ ((r >> 1 & 1) | (r >> 4 & 3) << 1);
+      const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ spread((r >> 1 & 1) | (r >> 4 & 3) << 1);
       w_off[j] = (uint32_t)r * (uint32_t)a.K + 16 * c;
       w_tail[j] = 16 * c >= last ? kPastEnd : 0u;
     } else {
@@ -254,7 +265,7 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(Dense
     const bool w_inside = OI ? (int64_t)(a.N - n0 - Tile::kCols) * a.K >= 16 : (int64_t)(a.K - (kb + 1) * kBlock) * a.N >= 16;
 #pragma unroll
     for (int j = 0; j < XL; ++j) {
-      const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ (r >> 1 & 7);
+      const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ spread(r >> 1 & 7);
       const int64_t at = (int64_t)min(m0 + r, a.M - 1) * a.K + min(kb * kBlock + 16 * c, a.K - 1);
       xg[j] = x_inside ? load16_any(a.x + at) : load16(a.x + at, x_total - at);
     }
@@ -262,7 +273,7 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(Dense
     for (int j = 0; j < WL; ++j) {
       int64_t at;
       if constexpr (OI) {
-        const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ ((r >> 1 & 1) | (r >> 4 & 3) << 1);
+        const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ spread((r >> 1 & 1) | (r >> 4 & 3) << 1);
         at = (int64_t)min(n0 + r, a.N - 1) * a.K + min(kb * kBlock + 16 * c, a.K - 1);
       } else {
         const int k = (64 / kLanesRow) * (wave + kWaves * j) + lane / kLanesRow;
@@ -277,13 +288,13 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(Dense
     if (block >= a.KB - 1 && last < kBlock) {  // the short last block: nothing past K
 #pragma unroll
       for (int j = 0; j < XL; ++j) {
-        const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ (r >> 1 & 7);
+        const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ spread(r >> 1 & 7);
         xg[j] = first_bytes(xg[j], last - 16 * c);
       }
 #pragma unroll
       for (int j = 0; j < WL; ++j) {
         if constexpr (OI) {
-          const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ ((r >> 1 & 1) | (r >> 4 & 3) << 1);
+          const int r = 8 * (wave + kWaves * j) + lane / 8, c = (lane % 8) ^ spread((r >> 1 & 1) | (r >> 4 & 3) << 1);
           wg[j] = first_bytes(wg[j], last - 16 * c);
         } else {
           const int k = (64 / kLanesRow) * (wave + kWaves * j) + lane / kLanesRow;
@@ -297,38 +308,44 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(Dense
     for (int j = 0; j < WL; ++j) *(lds_u32x4_rw*)(base + Tile::kW + buf * Tile::kWBytes + 1024 * (wave + kWaves * j) + 16 * lane) = wg[j];
     *(lds_float_rw*)(s_to + buf * Tile::kScaleBytes + 4 * lane) = sg;
   };
-  // DMA: the last block's chunks past K are sent past the end.  (Blocks past the last are requested like any other, from
-  // wherever they lie, and not used.)
-  auto request = [&](int kb, uint32_t buf) __attribute__((always_inline)) {
-    const Resource xr = make_resource(xp + (int64_t)kb * kBlock, x_left - (int64_t)kb * kBlock);
-    const Resource sr = make_resource(sp + (int64_t)kb * s_step, s_left - (int64_t)kb * s_step);
+  // DMA: loads `from` to `to` of a wave's kLoads of a block.  The last block's chunks past K are sent past the end.  (Blocks
+  // past the last are requested like any other, from wherever they lie, and not used.)
+  auto request = [&](int kb, uint32_t buf, int from, int to) __attribute__((always_inline)) {
     const uint32_t in_last = kb == a.KB - 1 ? 0xffffffffu : 0u;
-#pragma unroll
-    for (int j = 0; j < XL; ++j)
-      lds_load16(xr, x_off[j] | (x_tail[j] & in_last), base + Tile::kX + buf * Tile::kXBytes + 1024 * (wave + kWaves * j));
     const int64_t moved = (int64_t)kb * kBlock * (OI ? 1 : a.N);
-    const Resource wr = make_resource(wp + moved, w_left - moved);
 #pragma unroll
-    for (int j = 0; j < WL; ++j)
-      lds_load16(wr, w_off[j] | (w_tail[j] & in_last), base + Tile::kW + buf * Tile::kWBytes + 1024 * (wave + kWaves * j));
-    lds_load4(sr, s_off, s_to + buf * Tile::kScaleBytes);
+    for (int j = from; j < to; ++j) {
+      if (j < XL) {
+        lds_load16(make_resource(xp + (int64_t)kb * kBlock, x_left - (int64_t)kb * kBlock), x_off[j] | (x_tail[j] & in_last),
+                   base + Tile::kX + buf * Tile::kXBytes + 1024 * (wave + kWaves * j));
+      } else if (j < XL + WL) {
+        lds_load16(make_resource(wp + moved, w_left - moved), w_off[j - XL] | (w_tail[j - XL] & in_last),
+                   base + Tile::kW + buf * Tile::kWBytes + 1024 * (wave + kWaves * (j - XL)));
+      } else {
+        lds_load4(make_resource(sp + (int64_t)kb * s_step, s_left - (int64_t)kb * s_step), s_off, s_to + buf * Tile::kScaleBytes);
+      }
+    }
   };
+  // Half-groups of a step, counted from its barrier, and the loads requested before half-group h.
+  constexpr int kHalves = 2 * TB, kLoads = Tile::kLoads;
+  auto loads_before = [](int h) constexpr { return (h * kLoads + kHalves - 1) / kHalves; };
+  constexpr int kBehind = (2 * kLast * kLoads + kHalves - 1) / kHalves;  // those behind the barrier
 
   // Operand reads.
   const int wn = wave / Tile::WM, wm = wave % Tile::WM;
-  const int x_row = 16 * TB * wm + i, x_first = (2 * g) ^ (i >> 1 & 7);
+  const int x_row = 16 * TB * wm + i, x_first = (2 * g) ^ spread(i >> 1 & 7);
   const uint32_t xa = base + Tile::kX + x_row * kBlock + 16 * x_first;
   uint32_t wa;
   if constexpr (OI) {
-    const int r = 64 * wn + 16 * (i / 4) + i % 4, first = (2 * g) ^ ((i % 4) / 2 | (i / 4) << 1);
+    const int r = 64 * wn + 16 * (i / 4) + i % 4, first = (2 * g) ^ spread((i % 4) / 2 | (i / 4) << 1);
     wa = base + Tile::kW + r * kBlock + 16 * first;
   } else {
     const int k = 32 * g + i / 2;
     wa = base + Tile::kW + k * Tile::kCols + 16 * ((4 * wn) ^ Tile::k_swizzle(k)) + 8 * (i % 2);
   }
   const uint32_t sxa = base + Tile::kScale + 4 * x_row, swa = base + Tile::kScale + 4 * Tile::kRows + 4 * (64 * wn / kBlock);
-  i32x8 wo[4], xo[kRing];
-  float sx[kRing];
+  i32x8 wo[4], xo[TB];
+  float sx[TB], sw, sw_next;
   auto read_w = [&](int c, uint32_t buf) __attribute__((always_inline)) {
     const uint32_t at = wa + buf * Tile::kWBytes;
     if constexpr (OI) {
@@ -341,8 +358,8 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(Dense
   };
   auto read_x = [&](int b, uint32_t buf) __attribute__((always_inline)) {
     const uint32_t at = xa + buf * Tile::kXBytes;
-    xo[b % kRing] = join(lds_read16(at + 16 * kBlock * b), lds_read16((at ^ 16) + 16 * kBlock * b));
-    sx[b % kRing] = lds_read_float(sxa + buf * Tile::kScaleBytes + 64 * b);
+    xo[b] = join(lds_read16(at + 16 * kBlock * b), lds_read16((at ^ 16) + 16 * kBlock * b));
+    sx[b] = lds_read_float(sxa + buf * Tile::kScaleBytes + 64 * b);
   };
 
   f32x4 acc[4][TB] = {}, t[2][4] = {};
@@ -352,30 +369,36 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(Dense
   {
     if constexpr (DMA) {
 #pragma unroll
-      for (int j = 0; j < Tile::BUF; ++j) request(kb0 + j, j);
-      wait_loads<(Tile::BUF - 1) * Tile::kLoads>();
+      for (int j = 0; j < Tile::BUF - 1; ++j) request(kb0 + j, j, 0, kLoads);
+      request(kb0 + Tile::BUF - 1, Tile::BUF - 1, 0, kBehind);
+      wait_loads<(Tile::BUF - 2) * kLoads + kBehind>();
     } else {
       fetch(kb0);
       stage(kb0, 0);
       fetch(kb0 + 1);
     }
     lds_barrier();
-    float sw = lds_read_float(swa);
+    sw_next = lds_read_float(swa);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) read_w(c, 0);
+    for (int c = 0; c < 4; ++c) {
+      read_w(c, 0);
+      if (!kAhead) wv[c].set(wo[c]);
+    }
 #pragma unroll
     for (int b = 0; b < kLast; ++b) read_x(b, 0);
-    uint32_t cur = 0;
+    uint32_t cur = 0, left = Tile::BUF - 1;  // the step's buffer and the one before it
     for (int kb = kb0; kb < kb1; ++kb) {
       const uint32_t next = cur + 1 == Tile::BUF ? 0 : cur + 1;
-      float sw_next = 0.0f;
+      sw = sw_next;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (kAhead) wv[c].set(wo[c]);
 #pragma unroll
       for (int b = 0; b < TB; ++b) {
         if (b == TB - kLast) {
           if constexpr (DMA) {
-            wait_loads<(Tile::BUF - 2) * Tile::kLoads>();
+            wait_loads<(Tile::BUF - 2) * kLoads>();
             lds_barrier();
-            request(kb + Tile::BUF, cur);
           } else {
             stage(kb + 1, next);
             lds_barrier();
@@ -383,37 +406,47 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(Dense
           }
           sw_next = lds_read_float(swa + next * Tile::kScaleBytes);
         }
-        if (b + kLast < TB)
-          read_x(b + kLast, cur);
-        else
-          read_x(b + kLast - TB, next);
-        st[b % 2] = sx[b % kRing] * sw;
-        if (b == 0) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) wv[c].set(wo[c]);
-        }
         Operand<WIDE> xv;
-        xv.set(xo[b % kRing]);
+        xv.set(xo[b]);
+        st[b % 2] = sx[b] * sw;
+        const int p = b == 0 ? TB - 1 : b - 1;  // the group before (of the step before: t starts as zeros)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          t[b % 2][c] = block_sum(wv[c], xv);
-          if (b == TB - 1) read_w(c, next);
+        for (int h = 0; h < 2; ++h) {
+          if (b + kLast < TB) {
+            if (h == 0) read_x(b + kLast, cur);
+          } else {
+            if (h == 0) read_x(b + kLast - TB, next);
+            if (kAhead) read_w(2 * (b + kLast - TB) + h, next);
+          }
+#pragma unroll
+          for (int c = 2 * h; c < 2 * h + 2; ++c) t[b % 2][c] = block_sum(wv[c], xv);
+          if (!kAhead && b == TB - 1) {
+#pragma unroll
+            for (int c = 2 * h; c < 2 * h + 2; ++c) {
+              read_w(c, next);
+              wv[c].set(wo[c]);
+            }
+          }
+#pragma unroll
+          for (int c = 2 * h; c < 2 * h + 2; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[c][p][r] = fmaf(t[1 - b % 2][c][r], st[1 - b % 2], acc[c][p][r]);
+#pragma unroll
+          for (int c = 0; c < (WIDE ? 8 : 2); ++c) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+            __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);  // LDS read
+            __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // VALU
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (DMA) {
+            const bool behind = b >= TB - kLast;
+            const int at = 2 * (behind ? b - (TB - kLast) : b + kLast) + h;
+            request(behind ? kb + Tile::BUF : kb + Tile::BUF - 1, behind ? cur : left, loads_before(at), loads_before(at + 1));
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
-        constexpr int kBefore = TB - 1;
-        const int p = b == 0 ? kBefore : b - 1;  // the group before (of the step before: t starts as zeros)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[c][p][r] = fmaf(t[1 - b % 2][c][r], st[1 - b % 2], acc[c][p][r]);
-#pragma unroll
-        for (int c = 0; c < (WIDE ? 16 : 4); ++c) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
-          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS read
-          __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // VALU
-        }
-        __builtin_amdgcn_sched_barrier(0);
       }
-      sw = sw_next;
+      left = cur;
       cur = next;
     }
 #pragma unroll
@@ -422,7 +455,6 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(Dense
       for (int r = 0; r < 4; ++r) acc[c][TB - 1][r] = fmaf(t[1][c][r], st[1], acc[c][TB - 1][r]);
     if constexpr (DMA) wait_loads<0>();  // of the blocks past the last: LDS is the next workgroup's when this one ends
   }
-  static_assert(TB % 2 == 0, "the last group's sums lie in t[1]");
   if (a.S > 1) {
     // The slices' sums meet in scratch, stored and loaded with the agent-scope coherence bit (sc1): the slices may run
     // on different XCDs.  The last to arrive adds them in order and goes on; it leaves the counter at zero.
