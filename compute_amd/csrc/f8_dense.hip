@@ -26,10 +26,10 @@ struct DenseChoice {
 // slices, bfloat16 results)
 //   [97,4096] x 14336     128x128 in two 21.1, 64x128 21.9, 128x64 22.3, 256x128 in three 24.8
 //   [256,4096] x 4096     128x64 in two 16.5, 64x128 in two 16.7, 128x128 in three 17.3
-//   [512,4096] x 11008    256x128 42.2, 256x256 in two 51.9, 128x128 58.4
-//   [2048,4096] x 4096    256x128 42.6, 128x128 59.6, 256x256 60.5
-//   [4096,4096] x 4096    256x256 68.5 (2.0 PFLOP/s), 256x128 83.7, 128x128 116
-//   [2048,4096] x 14336   256x256 134, 256x128 167, 128x128 212
+//   [512,4096] x 11008    256x128 39.4, 256x256 in two 48.9, 128x128 59.1
+//   [2048,4096] x 4096    256x128 42.2, 256x256 54.7, 128x128 59.3
+//   [4096,4096] x 4096    256x256 66.5 (2.07 PFLOP/s), 256x128 82.8, 128x128 118
+//   [2048,4096] x 14336   256x256 126, 256x128 162, 128x128 216
 struct TileCost {
   int cols, rows, slots;  // workgroups at once on 256 CUs
   float step, wide_step;  // (float32 results)
@@ -37,8 +37,8 @@ struct TileCost {
   bool staged;              // also built for chunks through registers
 };
 constexpr float kNever = 1e9f;  // not built: bfloat16 operands of eight groups have no registers
-constexpr TileCost kTileCosts[] = {{256, 256, 256, 1.96f, kNever, 1.96f, kNever, false},
-                                   {256, 128, 256, 1.13f, 2.05f, 1.13f, 2.05f, false},
+constexpr TileCost kTileCosts[] = {{256, 256, 256, 1.82f, kNever, 1.82f, kNever, false},
+                                   {256, 128, 256, 1.10f, 2.05f, 1.10f, 2.05f, false},
                                    {128, 128, 256, 0.73f, 1.34f, 0.58f, 1.15f, true},
                                    {128, 64, 256, 0.50f, 0.82f, 0.44f, 0.76f, true},
                                    {64, 128, 256, 0.50f, 0.82f, 0.43f, 0.74f, false},

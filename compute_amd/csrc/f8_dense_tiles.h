@@ -53,7 +53,7 @@ namespace {
 // groups, whose operands are in registers: behind it begin the requests of the step BUF ahead, into the buffer just left, and
 // under those groups travel the first operands of the next step, all of w's among them (in registers of their own, from
 // which a step's start takes them; eight groups have too few registers left and read w's into place after their last use).
-// The requests are spread over the half-groups of a whole step: a wave stands still until its load is taken, 16 cycles each,
+// The requests are spread over half-groups: a wave stands still until its load is taken, 16 cycles each,
 // and 48 KB requested at once by all waves kept the MFMAs waiting for 780 cycles of a step of 2500 (1.04 us a step of 256 x 128 on one
 // CU, 0.85 when spread; the loads alone run at 152 GB/s a CU).
 struct Resource {
@@ -326,10 +326,14 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(Dense
       }
     }
   };
-  // Half-groups of a step, counted from its barrier, and the loads requested before half-group h.
-  constexpr int kHalves = 2 * TB, kLoads = Tile::kLoads;
-  auto loads_before = [](int h) constexpr { return (h * kLoads + kHalves - 1) / kHalves; };
-  constexpr int kBehind = (2 * kLast * kLoads + kHalves - 1) / kHalves;  // those behind the barrier
+  // Loads requested before half-group h of a step, counted from its barrier.  The last should have time to land before
+  // the next barrier and none to wait for the one before it (us; half-groups that carry loads):
+  //   256 x 256, two buffers    16: 137, 12: 133, 9: 127, 8: 128, 7: 129    [2048,4096] x 14336
+  //   256 x 128, three          8: 137, 7: 136, 5: 127, 4: 131, 3: 134      [2048,14336] x 4096
+  //   64 x 128, four            4: 21.4, 3: 22.8, 2: 22.5                   [97,4096] x 14336
+  constexpr int kSpread = TB == 2 ? 4 : TB == 4 ? 5 : 9, kLoads = Tile::kLoads;
+  auto loads_before = [](int h) constexpr { return h < kSpread ? (h * kLoads + kSpread - 1) / kSpread : kLoads; };
+  constexpr int kBehind = loads_before(2 * kLast);  // those behind the barrier
 
   // Operand reads.
   const int wn = wave / Tile::WM, wm = wave % Tile::WM;

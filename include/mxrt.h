@@ -501,7 +501,9 @@ int mx_quantized_embedding_lookup(mx_backend* b, const mx_qembed_args* args);
  * The operators on 8-bit floating-point blocks on device pointers (the Executable launches the same
  * kernels), on the backend's stream, asynchronous.  Arrays are contiguous; outputs must not overlap
  * inputs, except that dz may be dy itself.  Rows and columns are below 2^30.  mx_f8_dense with float x
- * takes the codes' memory from the backend's pool; the other calls allocate nothing.
+ * takes the codes' memory from the backend's pool; mx_f8_dense and mx_f8_weight_gradient that cut their sum into
+ * slices keep the slices' sums in the backend's scratch, which grows to the largest it was asked for (64 MB and
+ * 64 KB at most); the other calls allocate nothing.
  * ------------------------------------------------------------------------------------------- */
 typedef struct mx_f8_quantize_args {
   const void* x;      /* [M, K], x_dtype                                                      */

@@ -188,6 +188,73 @@ def test_dense(backend, M, K, N, oi, out):
     assert_within(run_dense(backend, x, xs, w, ws, oi, 0, out), want, bound, f"{M}x{K}x{N}")
 
 
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("oi", [True, False])
+@pytest.mark.parametrize("M,K,N", [(3390, 1040, 3600), (1000, 2320, 2064), (2050, 1296, 4368)])
+def test_dense_many_steps_and_tiles(backend, M, K, N, oi, out):
+    """Sampled rows of products of many tiles and blocks, the rows of the last tiles among them."""
+    x, xs, w, ws, _ = dense_problem(M, K, N, oi)
+    rows = np.unique(np.concatenate([np.random.default_rng(1).integers(0, M, 40), np.arange(M - 8, M), [0, 255, 256]]))
+    want, bound = dense_bound(x[rows], xs[rows], w, ws, oi, K, N, 0, out)
+    assert_within(run_dense(backend, x, xs, w, ws, oi, 0, out)[rows], want, bound, f"{M}x{K}x{N}")
+
+
+def dense_executable(backend, M, K, N, oi, out, seed):
+    """An executable of a product (of float x), its uploaded inputs."""
+    x, xs, w, ws, _ = dense_problem(M, K, N, oi, seed)
+    bld = backend.Builder("dense")
+    f = bld.Main()
+    arrays = {"x": (R.values(x, xs).astype(np.float32), F32), "w": (w, F8), "ws": (ws, F32)}
+    p = {n: f.Parameter(n, ca.Shape(dt, *a.shape)) for n, (a, dt) in arrays.items()}
+    f.Return([f.FusedF8Dense(p["x"], None, p["w"], p["ws"], None, ca.F8DenseConfig(0, int(oi), out))])
+    return bld.Compile(), [upload(backend, a, dt, *a.shape) for a, dt in arrays.values()]
+
+
+# Products whose K is cut into slices by the rule, of different sizes, and one that is not.
+SLICED = [(40, 4096, 512, True, F32), (97, 2048, 640, True, BF16), (24, 8192, 256, False, BF16), (600, 256, 512, True, BF16)]
+
+
+def test_dense_slices_repeat_bit_for_bit(backend):
+    """Sums that meet in scratch are added in one order: equal bits, also with other products between and a
+    scratch that has grown meanwhile."""
+    runs = [dense_executable(backend, *shape, seed) for seed, shape in enumerate(SLICED)]
+    first = [exe.Execute(inputs)[0].ToFlatData() for exe, inputs in runs]
+    for _ in range(8):
+        outs = [exe.Execute(inputs)[0] for exe, inputs in runs + runs[::-1]]
+        for o, want in zip(outs, first + first[::-1]):
+            assert np.array_equal(o.ToFlatData(), want)
+            o.Finalize()
+
+
+def test_dense_from_threads_and_two_backends(backend):
+    """Four threads, two on each of two backends, run sliced products at once: each gets its own results."""
+    import threading
+
+    other = ca.New("mi355x")
+    try:
+        runs = [dense_executable(b, *SLICED[i], i) for b in (backend, other) for i in range(2)]
+        want = [exe.Execute(inputs)[0].ToFlatData() for exe, inputs in runs]
+        assert np.array_equal(want[0], want[2]) and np.array_equal(want[1], want[3])
+        wrong = []
+
+        def work(exe, inputs, w):
+            for _ in range(30):
+                o, = exe.Execute(inputs)
+                if not np.array_equal(o.ToFlatData(), w):
+                    wrong.append(w.shape)
+                o.Finalize()
+
+        threads = [threading.Thread(target=work, args=(exe, inputs, w)) for (exe, inputs), w in zip(runs, want)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not wrong
+    finally:
+        del runs
+        other.Finalize()
+
+
 @pytest.mark.parametrize("act", range(6))
 @pytest.mark.parametrize("M,K,N,oi,b_dt,out", [(4, 300, 200, True, F32, F32), (4, 512, 256, True, BF16, BF16), (140, 256, 384, False, BF16, F32),
                                                (300, 512, 512, True, F32, BF16)])
