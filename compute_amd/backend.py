@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import enum
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Any, Optional, Sequence
 
 import numpy as np
@@ -226,6 +226,7 @@ class Capabilities:
     DTypes: dict
     Functions: bool = False
     DynamicAxes: bool = False
+    Extensions: dict = field(default_factory=dict)  # supported operators beyond the reference's enum
 
 
 # ---------------------------------------------------------------------------------------------
@@ -308,17 +309,17 @@ class Backend:
         return self._str(self._lib.mx_backend_device_description, device)
 
     def Capabilities(self) -> Capabilities:
-        ops, dts = {}, {}
+        ops, extensions, dts = {}, {}, {}
         v = C.c_int()
         for op in OpType:
             _check(self._lib.mx_backend_supports_op(self._h, int(op), C.byref(v)))
             if v.value:
-                ops[op] = True
+                (extensions if op >= OpType.F8Quantize else ops)[op] = True
         for dt in DType:
             _check(self._lib.mx_backend_supports_dtype(self._h, int(dt), C.byref(v)))
             if v.value:
                 dts[dt] = True
-        return Capabilities(Operations=ops, DTypes=dts)
+        return Capabilities(Operations=ops, DTypes=dts, Extensions=extensions)
 
     def HasSharedBuffers(self) -> bool:
         v = C.c_int()
