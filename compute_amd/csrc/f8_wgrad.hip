@@ -414,7 +414,8 @@ int run_tiles(mx_backend* b, const char* name, WGradArgs a, bool whole, int slic
 
 using Tile256 = Tile<4, 2, 2, 4, 64, 2>;
 using Tile128 = Tile<2, 2, 2, 2, 64, 2>;
-using TileF32 = Tile<2, 2, 2, 2, 32, 2>;
+using Tile256F32 = Tile<4, 2, 2, 4, 32, 2>;  // steps of 32 tokens: LDS holds dy three times
+using Tile128F32 = Tile<2, 2, 2, 2, 32, 2>;
 
 struct Choice {
   bool large;  // 256 x 256 tiles
@@ -428,13 +429,15 @@ struct Choice {
 //         2048 x 4096 x 4096      69 |  87          333 x 1536 x 384     -  | 9.7 12 12 12 16 16
 //         2048 x 2048 x 2048      -  |  31 34 42
 //   f32    333 x 1536 x 384       18.0 16.5 15.6 16.2 18.0 17.9    4000 x 512 x 512     148 79 57 47 38 35 (34 in 12)
-//         2048 x 2048 x 2048      85.8 75.6 82.8
+//         2048 x 2048 x 2048      155 | 85.8 75.6 82.8
+//         2048 x 4096 x 14336    701 | 842              515 x 7552 x 10528   290 | 362
+//         4096 x 4096 x 4096     353 | 461               63 x 7808 x 7296     78 | 62
 // Tiles of 128 x 256 and 256 x 128, two workgroups a CU, took 291 and 294 us for the first.
 Choice plan_of(const F8WGradDesc& d) {
   const bool f32 = d.dy_dt == MX_DTYPE_FLOAT32;
   Choice best{false, 1};
   double least = 1e30;
-  for (int large = 0; large < (f32 ? 1 : 2); ++large) {
+  for (int large = 0; large < 2; ++large) {
     const int side = large ? 256 : 128, S = f32 ? 32 : 64, slots = large ? 256 : 512;
     const int64_t tiles = ((d.K + side - 1) / side) * ((d.N + side - 1) / side), steps = (d.M + S - 1) / S;
     for (int slices = 1; slices <= 16 && slices <= std::max<int64_t>(steps, 1); ++slices) {
@@ -442,7 +445,7 @@ Choice plan_of(const F8WGradDesc& d) {
       const double part = (double)tiles * slices * side * side * 4;
       if (slices > 1 && ((steps + per - 1) / per != slices || tiles > (int64_t)(kCounterBytes / 4) || part > 64e6)) continue;
       const bool alone = tiles * slices <= 256;  // at most one workgroup a CU
-      const double step = large ? 1.72 : f32 ? (alone ? 1.28 : 1.9) : alone ? 0.83 : 1.2;
+      const double step = large ? (f32 ? 2.6 : 1.72) : f32 ? (alone ? 1.28 : 1.9) : alone ? 0.83 : 1.2;
       const double us = 3 + (double)((tiles * slices + slots - 1) / slots) * ((large ? 11 : alone ? 2 : 5) + (double)per * step) + (slices > 1 ? 3 + 1.2 * slices : 0);
       if (us < least) {
         least = us;
@@ -464,7 +467,8 @@ int f8_wgrad_run(mx_backend* b, const F8WGradDesc& d) {
   const bool whole = d.K % 16 == 0 && d.N % 8 == 0 && d.K <= 1 << 24 && d.N <= 1 << 24 && aligned16(d.x) && aligned16(d.dy);
   const char* name = f8_wgrad_name(d);
   const Choice c = plan_of(d);
-  if (d.dy_dt == MX_DTYPE_FLOAT32) return run_tiles<TileF32, true>(b, name, a, whole, c.slices);
+  if (d.dy_dt == MX_DTYPE_FLOAT32)
+    return c.large ? run_tiles<Tile256F32, true>(b, name, a, whole, c.slices) : run_tiles<Tile128F32, true>(b, name, a, whole, c.slices);
   return c.large ? run_tiles<Tile256, false>(b, name, a, whole, c.slices) : run_tiles<Tile128, false>(b, name, a, whole, c.slices);
 }
 

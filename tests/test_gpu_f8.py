@@ -409,6 +409,18 @@ def test_weight_gradient(backend, M, K, N, dt, oi, out):
 
 
 @pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("M,K,N,oi", [(200, 4112, 3408, True), (200, 4101, 3401, False), (333, 3600, 3592, False)])
+def test_weight_gradient_of_many_tiles(backend, M, K, N, oi, dt):
+    rng = np.random.default_rng(M + K)
+    x, xs = R.quantize(activations(rng, M, K))
+    dy = store(0.01 * activations(rng, M, N), dt)
+    want, bound = wgrad_want(x, xs, to_f64(dy, dt), oi, F32, dt)
+    cfg = (ca.DenseLayout(int(oi)), F32)
+    got, = run_graph(backend, lambda f, p: [f.FusedF8WeightGradient(p["x"], p["xs"], p["dy"], *cfg)], {"x": (x, F8), "xs": (xs, F32), "dy": (dy, dt)})
+    assert_within(got.astype(np.float64), want, bound, f"{M}x{K}x{N}")
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
 @pytest.mark.parametrize("M,K,N", [(40, 300, 200), (256, 256, 256)])
 def test_weight_gradient_any_scale(backend, M, K, N, dt):
     rng = np.random.default_rng(K)
