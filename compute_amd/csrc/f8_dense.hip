@@ -8,9 +8,9 @@ using namespace f8;
 
 using Tile256x256 = DenseTile<4, 2, 8, 2>;  // columns x rows
 using Tile256x128 = DenseTile<4, 2, 4, 3>;
-using Tile128x128 = DenseTile<2, 4, 2, 3>;  // (one more buffer makes the smaller tiles slower by up to 5%)
-using Tile128x64 = DenseTile<2, 2, 2, 4>;
-using Tile64x128 = DenseTile<1, 4, 2, 4>;
+using Tile128x128 = DenseTile<2, 4, 2, 3>;  // (with one more buffer the smaller tiles are up to 5% slower)
+using Tile128x64 = DenseTile<2, 2, 2, 3>;   // three: two workgroups a CU
+using Tile64x128 = DenseTile<1, 4, 2, 3>;
 using Tile64x64 = DenseTile<1, 2, 2, 4>;
 
 enum class DensePlan { kSkinny, kTiles, kStaged };
@@ -22,10 +22,10 @@ struct DenseChoice {
 // The tile and the number of K slices that take the least time by the measured times of their parts: a launch 3 us; a
 // round of workgroups its first loads and its stores 4.5 us, and a step of 128 k (below, us, with every CU at work); for sums
 // that meet in scratch 1.2 us, 0.3 us a slice and their bytes, out and back, at 14 TB/s (they mostly stay in the
-// caches).  Against sweeps of all of them at 20 shapes the choice is within 8% of the best, once 15% off, for instance (us, columns x rows,
+// caches).  Against sweeps of all of them at 28 shapes the choice is within 8% of the best, for instance (us, columns x rows,
 // slices, bfloat16 results)
-//   [97,4096] x 14336     128x128 in two 21.1, 64x128 21.9, 128x64 22.3, 256x128 in three 24.8
-//   [256,4096] x 4096     128x64 in two 16.5, 64x128 in two 16.7, 128x128 in three 17.3
+//   [97,4096] x 14336     128x128 in two 21.4, 64x128 in two 21.8, 64x128 22.3, 256x128 in three 24.8
+//   [256,4096] x 4096     128x64 in two 16.3, 64x128 in two 16.8, 128x128 in three 17.3
 //   [512,4096] x 11008    256x128 39.4, 256x256 in two 48.9, 128x128 59.1
 //   [2048,4096] x 4096    256x128 42.2, 256x256 54.7, 128x128 59.3
 //   [4096,4096] x 4096    256x256 66.5 (2.07 PFLOP/s), 256x128 82.8, 128x128 118
@@ -39,9 +39,9 @@ struct TileCost {
 constexpr float kNever = 1e9f;  // not built: bfloat16 operands of eight groups have no registers
 constexpr TileCost kTileCosts[] = {{256, 256, 256, 1.82f, kNever, 1.82f, kNever, false},
                                    {256, 128, 256, 1.10f, 2.05f, 1.10f, 2.05f, false},
-                                   {128, 128, 256, 0.73f, 1.34f, 0.58f, 1.15f, true},
-                                   {128, 64, 256, 0.50f, 0.82f, 0.44f, 0.76f, true},
-                                   {64, 128, 256, 0.50f, 0.82f, 0.43f, 0.74f, false},
+                                   {128, 128, 256, 0.73f, 1.34f, 0.58f, 1.20f, true},
+                                   {128, 64, 512, 0.80f, 1.15f, 0.44f, 0.76f, true},
+                                   {64, 128, 512, 0.80f, 1.15f, 0.43f, 0.74f, false},
                                    {64, 64, 512, 0.65f, 1.05f, 0.40f, 0.68f, true}};
 
 DenseChoice dense_plan(const F8DenseDesc& d) {
