@@ -12,6 +12,7 @@
 #include <algorithm>
 
 #include "f8_common.h"
+#include "f8_wgrad_schedule.h"
 #include "mxrt_internal.h"
 
 namespace mx {
@@ -50,13 +51,6 @@ __device__ __forceinline__ void parts_of(float v, uint16_t (&p)[3]) {
   p[2] = (uint16_t)(__float_as_uint(r2) >> 16);
 }
 
-// A workgroup computes kK (k) x kN (n) in WK x WN waves of 32 TK x 32 TN; tokens in steps of S.
-template <int WK_, int WN_, int TK_, int TN_, int S_, int OCC>
-struct Tile {
-  static constexpr int WK = WK_, WN = WN_, TK = TK_, TN = TN_, S = S_, kThreads = 64 * WK * WN, kOccupancy = OCC;
-  static constexpr int kK = 32 * TK * WK, kN = 32 * TN * WN, kPartBytes = 4 * kK * kN;
-};
-//
 // Staging.  The codes and dy of a step travel through registers, requested a step ahead: 16 codes a chunk,
 // scaled to bf16 (32 bytes of LDS), and 8 values of dy.  LDS keeps both as they lie in memory,
 // [token][column], in two buffers; the operands, eight consecutive tokens of a column per lane, come out
@@ -64,9 +58,9 @@ struct Tile {
 // 2 (token & 3), so that the 32 lanes of a half-wave, which read four rows of two neighbouring pieces,
 // touch every bank once.
 //
-// Schedule.  A step is G groups of TK MFMAs, one operand of dy against the wave's TK operands of x.  An
-// operand of dy is read kRing - 1 groups ahead of its use and the x operands of the next 16 tokens
-// during the present ones.  The step's barrier stands before its last kRing - 1 groups, whose operands
+// Schedule (f8_wgrad_schedule.h).  A step is groups of TK MFMAs, one operand of dy against the wave's TK operands of x.  An
+// operand of dy is read kLast groups ahead of its use and the x operands of the next 16 tokens
+// during the present ones.  The step's barrier stands before its last kLast groups, whose operands
 // are then in registers: under them travel the first operands of the next step.  A chunk of the next step
 // is staged, and that of the step after requested into its registers, in the groups before the barrier.
 //
@@ -90,26 +84,20 @@ struct Window {
   }
 };
 
-template <class Tile, bool F32, bool OI, bool WHOLE>
+template <class Tile, bool OI, bool WHOLE>
 __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_kernel(WGradArgs a) {
-  constexpr int TK = Tile::TK, TN = Tile::TN, S = Tile::S, kThreads = Tile::kThreads;
-  constexpr int P = F32 ? 3 : 1, WX = Tile::kK, WD = Tile::kN;  // parts of dy, columns of the operands
+  constexpr int TK = Tile::TK, TN = Tile::TN, S = Tile::S, P = Tile::P, kThreads = Tile::kThreads;
+  constexpr bool F32 = P == 3;
+  constexpr int WX = Tile::kK, WD = Tile::kN;          // columns of the operands
   constexpr int kXRow = 2 * WX, kDRow = 2 * WD;        // bytes of a row in LDS
   constexpr int kXBuf = S * kXRow, kDBuf = S * kDRow;  // x and a part of dy of a step
   constexpr int kStep = kXBuf + P * kDBuf;             // LDS of a step
-  constexpr int CX = S * WX / 16 / kThreads;           // chunks of x a thread stages
-  constexpr int CD = S * WD / 8 / kThreads;            // chunks of dy
+  constexpr int CX = Tile::kXChunks, CD = Tile::kDChunks;  // chunks of x and dy that a thread stages
   constexpr int RX = kThreads / (WX / 16), RD = kThreads / (WD / 8);  // rows between a thread's chunks
-  constexpr int kParts = S / 16, kPart = P * TN, G = kParts * kPart;
-  constexpr int kRing = 4, kLast = kRing - 1;          // groups after the barrier
-  constexpr int kPieces = 2 * CX + CD;                 // staged at a time: half a chunk of x or one of dy, mixed evenly
+  constexpr int kParts = Tile::kParts, kPart = Tile::kPart, G = Tile::kGroups, kRing = Tile::kRing, kLast = Tile::kLast;
+  constexpr int kPieces = Tile::kPieces;
   auto x_before = [](int p) constexpr { return (p * 2 * CX + kPieces - 1) / kPieces; };  // pieces of x among the first p
-  constexpr int kStageGroups = G - kLast < kPieces ? G - kLast : kPieces, kStageFrom = G - kLast - kStageGroups;
-  constexpr int kPerGroup = (kPieces + kStageGroups - 1) / kStageGroups;
   constexpr int H = F32 ? 2 : 1, E = F32 ? 4 : 2;      // loads of a dy chunk, bytes of a value
-  static_assert(CX * 16 * kThreads == S * WX && CD * 8 * kThreads == S * WD, "whole chunks");
-  static_assert(kParts % 2 == 0 && kPart >= TK, "the sets of x operands alternate, and one is read while the other is used");
-  static_assert(G % kRing == 0, "the ring's slots are the same in every step");
   static_assert(kStep % 1024 == 0, "the buffers differ above the bits of a piece");
   static_assert((TK & (TK - 1)) == 0 && (TN & (TN - 1)) == 0, "a wave's pieces start on a multiple of their number: an XOR picks one");
   extern __shared__ __align__(1024) uint8_t lds[];     // [2]: x [S][WX], then the parts of dy [P][S][WD], bf16
@@ -254,26 +242,30 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_ker
 #pragma unroll
       for (int q = 0; q < G; ++q) {
         const int part = q / kPart, set = part % 2;
-        if (q == G - kLast) lds_barrier();
+        if (q == Tile::kBarrier) lds_barrier();
         // Operands of later groups.
         if (q + kLast < G)
           read_dy(q + kLast, cur);
         else
           read_dy(q + kLast - G, next);
-        if (part + 1 < kParts && q % kPart < TK) read_x(1 - set, q % kPart, cur, part + 1);
-        constexpr int kTail = kLast < kPart ? kLast : kPart;  // groups of the last 16 tokens behind the barrier
-        if (q >= G - kTail) {
-          constexpr int per = (TK + kTail - 1) / kTail;
+        if (part + 1 < kParts && q % kPart < Tile::kXGroups) {
 #pragma unroll
-          for (int e = 0; e < per; ++e) {
-            const int t = (q - (G - kTail)) * per + e;
+          for (int e = 0; e < Tile::kXPer; ++e) {
+            const int t = q % kPart * Tile::kXPer + e;
+            if (t < TK) read_x(1 - set, t, cur, part + 1);
+          }
+        }
+        if (q >= G - Tile::kNextGroups) {
+#pragma unroll
+          for (int e = 0; e < Tile::kNextPer; ++e) {
+            const int t = (q - (G - Tile::kNextGroups)) * Tile::kNextPer + e;
             if (t < TK) read_x(0, t, next, 0);
           }
         }
-        if (q >= kStageFrom && q < G - kLast) {
+        if (q >= Tile::kStageFrom && q < Tile::kBarrier) {
 #pragma unroll
-          for (int e = 0; e < kPerGroup; ++e) {
-            const int p = (q - kStageFrom) * kPerGroup + e;
+          for (int e = 0; e < Tile::kPerGroup; ++e) {
+            const int p = (q - Tile::kStageFrom) * Tile::kPerGroup + e;
             if (p < kPieces) {
               stage(inside, m0 + S, next, p);
               request(inside, m0 + 2 * S, p);
@@ -391,9 +383,9 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_ker
 
 constexpr size_t kCounterBytes = 64 * 1024;  // of the backend's scratch: arrival counters, zero between launches
 
-template <class Tile, bool F32>
+template <class Tile>
 int run_tiles(mx_backend* b, const char* name, WGradArgs a, bool whole, int slices) {
-  constexpr int P = F32 ? 3 : 1, kLds = 2 * 2 * Tile::S * (Tile::kK + P * Tile::kN);
+  constexpr int kLds = 2 * 2 * Tile::S * (Tile::kK + Tile::P * Tile::kN);
   const int64_t tk = (a.K + Tile::kK - 1) / Tile::kK, tn = (a.N + Tile::kN - 1) / Tile::kN;
   const int steps = (a.M + Tile::S - 1) / Tile::S, per = (steps + slices - 1) / slices;
   a.tokens = std::max(per, 1) * Tile::S;
@@ -406,16 +398,11 @@ int run_tiles(mx_backend* b, const char* name, WGradArgs a, bool whole, int slic
     a.arrived = (uint32_t*)scratch;
     a.part = (char*)scratch + kCounterBytes;
   }
-  auto k = a.oi ? (whole ? f8_wgrad_kernel<Tile, F32, true, true> : f8_wgrad_kernel<Tile, F32, true, false>)
-                : (whole ? f8_wgrad_kernel<Tile, F32, false, true> : f8_wgrad_kernel<Tile, F32, false, false>);
+  auto k = a.oi ? (whole ? f8_wgrad_kernel<Tile, true, true> : f8_wgrad_kernel<Tile, true, false>)
+                : (whole ? f8_wgrad_kernel<Tile, false, true> : f8_wgrad_kernel<Tile, false, false>);
   MX_CHECK_HIP(hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
   return launch(b, name, [&] { dispatch(k, dim3((unsigned)(tk * tn * a.slices)), dim3(Tile::kThreads), kLds, b->stream, a); });
 }
-
-using Tile256 = Tile<4, 2, 2, 4, 64, 2>;
-using Tile128 = Tile<2, 2, 2, 2, 64, 2>;
-using Tile256F32 = Tile<4, 2, 2, 4, 32, 2>;  // steps of 32 tokens: LDS holds dy three times
-using Tile128F32 = Tile<2, 2, 2, 2, 32, 2>;
 
 struct Choice {
   bool large;  // 256 x 256 tiles
@@ -468,8 +455,8 @@ int f8_wgrad_run(mx_backend* b, const F8WGradDesc& d) {
   const char* name = f8_wgrad_name(d);
   const Choice c = plan_of(d);
   if (d.dy_dt == MX_DTYPE_FLOAT32)
-    return c.large ? run_tiles<Tile256F32, true>(b, name, a, whole, c.slices) : run_tiles<Tile128F32, true>(b, name, a, whole, c.slices);
-  return c.large ? run_tiles<Tile256, false>(b, name, a, whole, c.slices) : run_tiles<Tile128, false>(b, name, a, whole, c.slices);
+    return c.large ? run_tiles<WGradTile256F32>(b, name, a, whole, c.slices) : run_tiles<WGradTile128F32>(b, name, a, whole, c.slices);
+  return c.large ? run_tiles<WGradTile256>(b, name, a, whole, c.slices) : run_tiles<WGradTile128>(b, name, a, whole, c.slices);
 }
 
 }  // namespace mx
