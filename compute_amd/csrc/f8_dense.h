@@ -18,6 +18,7 @@ struct DenseArgs {
   int M, K, N, KB, NB;
   int b_dt, out_dt, act, oi;
   int tiles_n, vec_out;
+  int first;          // few rows: the launch's first strip of columns
   int S, kps;         // slices of K of a tile, blocks of a slice
   char* part;         // [tile][slice] sums (S > 1)
   uint32_t* arrived;  // [tile], zero between launches
@@ -45,7 +46,7 @@ __device__ __forceinline__ f32x4 block_sum(const i32x8& a, const i32x8& b) {
 inline DenseArgs dense_args(const F8DenseDesc& d) {
   const bool codes = d.x_dt == MX_DTYPE_F8E4M3FN;
   return DenseArgs{codes ? (const uint8_t*)d.x : nullptr, codes ? nullptr : d.x, d.x_scale, d.w, d.w_scale, d.bias, d.out,
-                   (int)d.M, (int)d.K, (int)d.N, (int)blocks(d.K), (int)blocks(d.N), d.b_dt, d.out_dt, d.act, d.oi, 0, 0, 1, 0, nullptr, nullptr};
+                   (int)d.M, (int)d.K, (int)d.N, (int)blocks(d.K), (int)blocks(d.N), d.b_dt, d.out_dt, d.act, d.oi, 0, 0, 0, 1, 0, nullptr, nullptr};
 }
 
 // Up to 16 rows, weights [N, K] (f8_skinny.hip); float x up to four rows.

@@ -31,18 +31,18 @@ struct DenseChoice {
 //   [4096,4096] x 4096    256x256 66.5 (2.07 PFLOP/s), 256x128 82.8, 128x128 118
 //   [2048,4096] x 14336   256x256 126, 256x128 162, 128x128 216
 struct TileCost {
-  int cols, rows, slots;  // workgroups at once on 256 CUs
+  int cols, rows, threads, slots;  // threads of a workgroup, workgroups at once on 256 CUs
   float step, wide_step;  // (float32 results)
   float alone, wide_alone;  // with at most one workgroup a CU
   bool staged;              // also built for chunks through registers
 };
 constexpr float kNever = 1e9f;  // not built: bfloat16 operands of eight groups have no registers
-constexpr TileCost kTileCosts[] = {{256, 256, 256, 1.82f, kNever, 1.82f, kNever, false},
-                                   {256, 128, 256, 1.10f, 2.05f, 1.10f, 2.05f, false},
-                                   {128, 128, 256, 0.73f, 1.34f, 0.58f, 1.20f, true},
-                                   {128, 64, 512, 0.80f, 1.15f, 0.44f, 0.76f, true},
-                                   {64, 128, 512, 0.80f, 1.15f, 0.43f, 0.74f, false},
-                                   {64, 64, 512, 0.65f, 1.05f, 0.40f, 0.68f, true}};
+constexpr TileCost kTileCosts[] = {{256, 256, 512, 256, 1.82f, kNever, 1.82f, kNever, false},
+                                   {256, 128, 512, 256, 1.10f, 2.05f, 1.10f, 2.05f, false},
+                                   {128, 128, 512, 256, 0.73f, 1.34f, 0.58f, 1.20f, true},
+                                   {128, 64, 256, 512, 0.80f, 1.15f, 0.44f, 0.76f, true},
+                                   {64, 128, 256, 512, 0.80f, 1.15f, 0.43f, 0.74f, false},
+                                   {64, 64, 128, 512, 0.65f, 1.05f, 0.40f, 0.68f, true}};
 
 DenseChoice dense_plan(const F8DenseDesc& d) {
   if (skinny_fits(d)) return {DensePlan::kSkinny, 0, 1};
@@ -60,6 +60,7 @@ DenseChoice dense_plan(const F8DenseDesc& d) {
     for (int S = 1; S <= 16 && S <= KB; ++S) {
       const int64_t per = (KB + S - 1) / S, used = (KB + per - 1) / per;  // slices that are not empty
       const double part = (double)tiles * (double)used * c.rows * c.cols * 4;
+      if (tiles * S * c.threads > kMaxWorkItems) continue;
       if (S > 1 && (used != S || tiles > (int64_t)(kCounterBytes / 4) || part > 64e6)) continue;
       const bool alone = tiles * S <= 256;
       const double step = wide ? (alone ? c.wide_alone : c.wide_step) : alone ? c.alone : c.step;

@@ -514,7 +514,7 @@ int run_dense_tiles(mx_backend* b, const char* name, DenseArgs a, int slices) {
   a.tiles_n = (int)tn;
   a.kps = std::max((a.KB + slices - 1) / slices, 1);
   a.S = std::max((a.KB + a.kps - 1) / a.kps, 1);  // K = 0: one slice without a block, act(bias)
-  if (tm * tn * a.S >= (int64_t)1 << 31) return set_error(MX_ERR_INVALID, "F8Dense: more than 2^31 workgroups");
+  if (tm * tn * a.S * Tile::kThreads > kMaxWorkItems) return set_error(MX_ERR_INVALID, "F8Dense: a result of more tiles than a launch holds");
   if (a.S > 1) {
     void* scratch = nullptr;
     MX_TRY(ensure_scratch(b, kCounterBytes + (size_t)(tm * tn * a.S) * Tile::kPartBytes, &scratch));

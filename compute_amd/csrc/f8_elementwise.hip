@@ -106,11 +106,12 @@ __device__ __forceinline__ uint32_t largest8(const float (&v)[8]) {
   return m;
 }
 
-// One scale per 128 values of a row: block t of the M * KB blocks is row t / KB's.
+// One scale per 128 values of a row: block t of the M * KB blocks is row t / KB's.  A launch holds the workgroups from
+// `first` on.
 template <bool F32, bool VEC>
 __global__ __launch_bounds__(kThreads) void f8_quantize_rows_kernel(const void* x, uint8_t* codes, float* scale, int K,
-                                                                    int KB, int64_t total) {
-  const int64_t t = (int64_t)blockIdx.x * kGroups + threadIdx.x / kLanes;
+                                                                    int KB, int64_t total, int64_t first) {
+  const int64_t t = (first + blockIdx.x) * kGroups + threadIdx.x / kLanes;
   if (t >= total) return;
   const int64_t row = t / KB;
   const int k0 = (int)(t - row * KB) * kBlock + (int)(threadIdx.x % kLanes) * kPerLane;
@@ -126,10 +127,11 @@ __global__ __launch_bounds__(kThreads) void f8_quantize_rows_kernel(const void* 
 // One scale per 128 x 128 block: a workgroup's, its values held in registers between the passes.
 template <bool F32, bool VEC>
 __global__ __launch_bounds__(kThreads) void f8_quantize_tiles_kernel(const void* x, uint8_t* codes, float* scale, int M,
-                                                                     int K, int KB) {
+                                                                     int K, int KB, unsigned first) {
   constexpr int kPasses = kBlock / kGroups;
   __shared__ uint32_t part[kThreads / 64];
-  const int rb = (int)(blockIdx.x / (unsigned)KB), cb = (int)(blockIdx.x % (unsigned)KB);
+  const unsigned at = first + blockIdx.x;  // fewer than 2^32 blocks in 2^45 values
+  const int rb = (int)(at / (unsigned)KB), cb = (int)(at % (unsigned)KB);
   const int k0 = cb * kBlock + (int)(threadIdx.x % kLanes) * kPerLane;
   const int n = K - k0;
   float v[kPasses][8];
@@ -226,12 +228,12 @@ struct ActGradArgs {
   const void* dy;
   void *dz, *dup;
   int N, NB;
-  int64_t total;  // blocks
+  int64_t total, first;  // blocks; the launch's first workgroup
 };
 
 template <bool F32, bool VEC, bool GATED, int ACT>
 __global__ __launch_bounds__(kThreads) void f8_act_grad_kernel(ActGradArgs a) {
-  const int64_t t = (int64_t)blockIdx.x * kGroups + threadIdx.x / kLanes;
+  const int64_t t = (a.first + blockIdx.x) * kGroups + threadIdx.x / kLanes;
   if (t >= a.total) return;
   const int64_t row = t / a.NB;
   const int n0 = (int)(t - row * a.NB) * kBlock + (int)(threadIdx.x % kLanes) * kPerLane;
@@ -264,9 +266,6 @@ auto act_grad_kernel(int act) {
   }
 }
 
-int grid_too_large(const char* op) { return set_error(MX_ERR_INVALID, "%s: more than 2^31 workgroups", op); }
-constexpr int64_t kMaxGrid = ((int64_t)1 << 31) - 1;
-
 bool aligned8(const void* p) { return ((uintptr_t)p & 7) == 0; }
 
 }  // namespace
@@ -278,19 +277,17 @@ int f8_quantize_run(mx_backend* b, const F8QuantizeDesc& d) {
   const int64_t KB = blocks(d.K);
   if (d.rows == 1) {
     const int64_t total = d.M * KB, grid = (total + kGroups - 1) / kGroups;
-    if (grid > kMaxGrid) return grid_too_large("F8Quantize");
     auto k = f32 ? (vec ? f8_quantize_rows_kernel<true, true> : f8_quantize_rows_kernel<true, false>)
                  : (vec ? f8_quantize_rows_kernel<false, true> : f8_quantize_rows_kernel<false, false>);
-    return launch(b, "f8_quantize_rows", [&] {
-      dispatch(k, dim3((unsigned)grid), dim3(kThreads), 0, b->stream, d.x, d.codes, d.scale, (int)d.K, (int)KB, total);
+    return launch_runs(b, "f8_quantize_rows", grid, kThreads, [&](int64_t first, unsigned count) {
+      dispatch(k, dim3(count), dim3(kThreads), 0, b->stream, d.x, d.codes, d.scale, (int)d.K, (int)KB, total, first);
     });
   }
   const int64_t grid = blocks(d.M) * KB;
-  if (grid > kMaxGrid) return grid_too_large("F8Quantize");
   auto k = f32 ? (vec ? f8_quantize_tiles_kernel<true, true> : f8_quantize_tiles_kernel<true, false>)
                : (vec ? f8_quantize_tiles_kernel<false, true> : f8_quantize_tiles_kernel<false, false>);
-  return launch(b, "f8_quantize_tiles", [&] {
-    dispatch(k, dim3((unsigned)grid), dim3(kThreads), 0, b->stream, d.x, d.codes, d.scale, (int)d.M, (int)d.K, (int)KB);
+  return launch_runs(b, "f8_quantize_tiles", grid, kThreads, [&](int64_t first, unsigned count) {
+    dispatch(k, dim3(count), dim3(kThreads), 0, b->stream, d.x, d.codes, d.scale, (int)d.M, (int)d.K, (int)KB, (unsigned)first);
   });
 }
 
@@ -299,14 +296,14 @@ int f8_act_grad_run(mx_backend* b, const F8ActGradDesc& d) {
   const bool f32 = d.dy_dt == MX_DTYPE_FLOAT32, gated = d.up != nullptr;
   const bool vec = d.N % kPerLane == 0 && aligned8(d.z) && aligned8(d.up) && aligned16(d.dy) && aligned16(d.dz) && aligned16(d.dup);
   const int64_t NB = blocks(d.N), total = d.M * NB, grid = (total + kGroups - 1) / kGroups;
-  if (grid > kMaxGrid) return grid_too_large("F8ActivationGradient");
-  const ActGradArgs a{d.z, d.up, d.z_scale, d.up_scale, d.dy, d.dz, d.dup, (int)d.N, (int)NB, total};
+  ActGradArgs a{d.z, d.up, d.z_scale, d.up_scale, d.dy, d.dz, d.dup, (int)d.N, (int)NB, total, 0};
   auto k = f32 ? (vec ? (gated ? act_grad_kernel<true, true, true>(d.act) : act_grad_kernel<true, true, false>(d.act))
                       : (gated ? act_grad_kernel<true, false, true>(d.act) : act_grad_kernel<true, false, false>(d.act)))
                : (vec ? (gated ? act_grad_kernel<false, true, true>(d.act) : act_grad_kernel<false, true, false>(d.act))
                       : (gated ? act_grad_kernel<false, false, true>(d.act) : act_grad_kernel<false, false, false>(d.act)));
-  return launch(b, gated ? "f8_act_grad_gated" : "f8_act_grad", [&] {
-    dispatch(k, dim3((unsigned)grid), dim3(kThreads), 0, b->stream, a);
+  return launch_runs(b, gated ? "f8_act_grad_gated" : "f8_act_grad", grid, kThreads, [&](int64_t first, unsigned count) {
+    a.first = first;
+    dispatch(k, dim3(count), dim3(kThreads), 0, b->stream, a);
   });
 }
 

@@ -33,7 +33,7 @@ __global__ __launch_bounds__(64 * NW) void f8_skinny_kernel(DenseArgs a) {
   __shared__ float scales[kFloat ? NW : 1][kFloatRows];
   __shared__ f32x4 sums[NW][C][64];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), i = lane % 16, g = lane / 16;
-  const int n0 = 16 * C * xcd_order((int)blockIdx.x, (int)gridDim.x);
+  const int n0 = 16 * C * (a.first + xcd_order((int)blockIdx.x, (int)gridDim.x));
   const uint8_t* wrow[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) wrow[c] = a.w + (int64_t)min(n0 + 16 * c + i, a.N - 1) * a.K + 32 * g;
@@ -169,10 +169,12 @@ __global__ __launch_bounds__(64 * NW) void f8_skinny_kernel(DenseArgs a) {
 // From 768 strips the CUs are full with two operands, which share the lanes' x (as many bytes as the weights with 16
 // rows); from 512 with four waves; below, the waves have to come from K, and with more rows their sums cost more.
 template <int X, bool WIDE>
-int run_skinny(mx_backend* b, const char* name, const DenseArgs& a) {
+int run_skinny(mx_backend* b, const char* name, DenseArgs a) {
   auto go = [&](auto k, int waves, int c) {
-    const int strips = (int)(((int64_t)a.N + 16 * c - 1) / (16 * c));
-    return launch(b, name, [&] { dispatch(k, dim3((unsigned)strips), dim3(64 * waves), 0, b->stream, a); });
+    return launch_runs(b, name, ((int64_t)a.N + 16 * c - 1) / (16 * c), 64 * waves, [&](int64_t first, unsigned count) {
+      a.first = (int)first;
+      dispatch(k, dim3(count), dim3(64 * waves), 0, b->stream, a);
+    });
   };
   const int strips = (int)(((int64_t)a.N + 15) / 16);
   if (a.M <= kFloatRows) {  // float rows and their codes alike: the same order of sums, the same bits

@@ -391,7 +391,8 @@ int run_tiles(mx_backend* b, const char* name, WGradArgs a, bool whole, int slic
   a.tokens = std::max(per, 1) * Tile::S;
   a.slices = std::max((a.M + a.tokens - 1) / a.tokens, 1);
   a.tiles_n = (int)tn;
-  if (tk * tn * a.slices >= (int64_t)1 << 31) return set_error(MX_ERR_INVALID, "F8WeightGradient: more than 2^31 workgroups");
+  if (tk * tn * a.slices * Tile::kThreads > kMaxWorkItems)
+    return set_error(MX_ERR_INVALID, "F8WeightGradient: a result of more tiles than a launch holds");
   if (a.slices > 1) {
     void* scratch = nullptr;
     MX_TRY(ensure_scratch(b, kCounterBytes + (size_t)(tk * tn * a.slices) * Tile::kPartBytes, &scratch));
@@ -430,6 +431,7 @@ Choice plan_of(const F8WGradDesc& d) {
     for (int slices = 1; slices <= 16 && slices <= std::max<int64_t>(steps, 1); ++slices) {
       const int64_t per = (steps + slices - 1) / slices;
       const double part = (double)tiles * slices * side * side * 4;
+      if (tiles * slices * (large ? WGradTile256::kThreads : WGradTile128::kThreads) > kMaxWorkItems) continue;
       if (slices > 1 && ((steps + per - 1) / per != slices || tiles > (int64_t)(kCounterBytes / 4) || part > 64e6)) continue;
       const bool alone = tiles * slices <= 256;  // at most one workgroup a CU
       const double step = large ? (f32 ? 2.6 : 1.72) : f32 ? (alone ? 1.28 : 1.9) : alone ? 0.83 : 1.2;

@@ -212,6 +212,20 @@ void dispatch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t lds, hipSt
                         static_cast<KArgs>(args)...);
 }
 
+// Work-items that a launch can have along a grid dimension.
+constexpr int64_t kMaxWorkItems = ((int64_t)1 << 32) - 1;
+
+// Workgroups 0 .. groups - 1 of `threads` each, in as many launches as that takes: fn(first, count).
+template <typename F>
+int launch_runs(mx_backend* b, const char* name, int64_t groups, int threads, F&& fn) {
+  const int64_t most = kMaxWorkItems / threads;
+  for (int64_t first = 0; first < groups; first += most) {
+    const unsigned count = (unsigned)(groups - first < most ? groups - first : most);
+    MX_TRY(launch(b, name, [&] { fn(first, count); }));
+  }
+  return MX_OK;
+}
+
 // ------------------------------------------------------------------------------------------
 // Kernel launchers (implemented in the .hip files).
 // ------------------------------------------------------------------------------------------
