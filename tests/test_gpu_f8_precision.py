@@ -1,9 +1,10 @@
-"""What mxrt.h promises of the sums of the dense product over 8-bit blocks, where ordinary data does not show it."""
+"""Precision of the operators on 8-bit blocks where ordinary data does not show it: sums that cancel, tails of activations."""
 import numpy as np
 import pytest
 
+import compute_amd as ca
 from oracle import f8_ref as R
-from tests.test_gpu_f8 import BF16, F32, assert_within, run_dense
+from tests.test_gpu_f8 import BF16, F8, F32, assert_within, run_dense, run_graph, store, to_f64
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +32,41 @@ def test_sums_that_cancel(backend, M, K, N, oi):
     got = run_dense(backend, codes, scale, w, ws, oi, 0, BF16)
     cut = K // 8 * 7 * 2.0 ** -13 * 256
     assert_within(got, want, np.full_like(want, cut) + 2.0 ** -8 * (np.abs(want) + cut), "bfloat16")
+
+
+@pytest.mark.parametrize("dt", [BF16, F32])
+@pytest.mark.parametrize("act", [1, 3])
+def test_activation_gradient_tails(backend, act, dt):
+    """GELU and SiLU far from zero, each result held against its own size, dz against the terms of its slope.
+
+    bfloat16: GELU's polynomial 3.8e-5, the exponent z^2 / 2 (SiLU: z) rounded twice, z^2 * 2^-24 <= 1.1e-5, and 16 roundings of
+    2^-24: below 2^-13; half a step of 2^-8.  float32: erfc's argument is rounded twice, which moves erfc by 1.5 z^2 * 2^-24, the
+    exponent's by z^2 * 2^-24 (SiLU: 2 |z| * 2^-24), erfc and exp to 8 ulp, 16 roundings: (3 z^2 + 32) 2^-24.
+    """
+    z = R.VALUES[[c for c in range(256) if (c & 127) != 127]]
+    z = np.concatenate([z * s for s in (2.0 ** -5, 2.0 ** -6, 2.0 ** -7)])
+    z = np.unique(z[(z >= -13) & (z != 0)])
+    z = np.resize(z, (-(-z.size // 128), 128))
+    codes, scale = R.quantize(z)
+    exact = R.values(codes, scale)
+    rng = np.random.default_rng(1)
+    dy = store(rng.uniform(0.5, 2, z.shape).astype(np.float32), dt)
+    ones, one = R.quantize(np.ones(z.shape))
+
+    def build(f, p):
+        return f.FusedF8ActivationGradient(p["z"], p["zs"], p["dy"], ca.ActivationType(act), p["u"], p["us"])
+
+    dz, dup = run_graph(backend, build, {"z": (codes, F8), "zs": (scale, F32), "dy": (dy, dt), "u": (ones, F8), "us": (one, F32)})
+    d = to_f64(dy, dt)
+    rel = 2.0 ** -13 if dt == BF16 else (3 * exact ** 2 + 32) * 2.0 ** -24
+    half = 2.0 ** -8 if dt == BF16 else 2.0 ** -24
+    want = d * R.act(exact, act)
+    assert_within(to_f64(dup, dt), want, (rel + half * (1 + rel)) * np.abs(want) + 1e-38, "dup")
+    # the slope's terms: the cumulative and z times the density (GELU), g and z g (1 - g) (SiLU)
+    if act == 1:
+        terms = R.act(exact, 1) / np.where(exact == 0, 1, exact) + np.abs(exact) * np.exp(-exact ** 2 / 2) / np.sqrt(2 * np.pi)
+    else:
+        g = 1 / (1 + np.exp(-exact))
+        terms = g + np.abs(exact) * g * (1 - g)
+    want = d * R.slope(exact, act)
+    assert_within(to_f64(dz, dt), want, rel * d * terms + half * np.abs(want) * 1.001 + 1e-38, "dz")
