@@ -65,7 +65,7 @@ __device__ __forceinline__ void parts_of(float v, uint16_t (&p)[3]) {
 // is staged, and that of the step after requested into its registers, in the groups before the barrier.
 //
 // Columns past K or N hold whatever lies there: they meet only results that are not stored.  Tokens past
-// M are zeros in both operands (a step past the last is staged like any other and not used).  WHOLE: rows
+// M are zeros in both operands, their scales too (a step past the last is staged like any other and not used).  WHOLE: rows
 // are whole chunks below 2^24 columns, read through buffer resources that end with the array, so that
 // what lies past it reads as zero; otherwise a chunk may start anywhere and run into the next row, and the
 // tokens and the array's end are looked at.
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_ker
     uint8_t* xb = lds + step;
     if (x_before(piece + 1) > x_before(piece)) {
       const int j = x_before(piece) / 2, half = x_before(piece) % 2;
-      if (kMask && half == 0 && m0 + xrow + j * RX >= to) xr[j] = u32x4{0u, 0u, 0u, 0u};
+      if (kMask && half == 0 && m0 + xrow + j * RX >= to) xr[j] = u32x4{0u, 0u, 0u, 0u}, sr[j] = 0.0f;
       u32x4 o;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {

@@ -4,7 +4,7 @@ import pytest
 
 import compute_amd as ca
 from oracle import f8_ref as R
-from tests.test_gpu_f8 import BF16, F8, F32, assert_within, run_dense, run_graph, store, to_f64
+from tests.test_gpu_f8 import BF16, F8, F32, assert_within, run_dense, run_graph, store, to_f64, wgrad_want
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +70,20 @@ def test_activation_gradient_tails(backend, act, dt):
         terms = g + np.abs(exact) * g * (1 - g)
     want = d * R.slope(exact, act)
     assert_within(to_f64(dz, dt), want, rel * d * terms + half * np.abs(want) * 1.001 + 1e-38, "dz")
+
+
+@pytest.mark.parametrize("M,K,N", [(37, 130, 70), (37, 144, 72), (700, 131, 45), (64, 144, 72)])
+@pytest.mark.parametrize("oi", [True, False])
+def test_weight_gradient_of_an_infinite_row(backend, M, K, N, oi):
+    """The last token's first block overflows: positive codes times positive dy are infinite there, and the tokens that
+    pad the last step, whose codes are zeros, add nothing to them; the second block is as ever."""
+    rng = np.random.default_rng(K)
+    x, xs = R.encode(np.full((M, K), 1.5)), np.ones((M, 2), np.float32)
+    xs[M - 1, 0] = np.inf
+    dy = store(rng.uniform(0.5, 1, (M, N)).astype(np.float32), BF16)
+    got, = run_graph(backend, lambda f, p: [f.FusedF8WeightGradient(p["x"], p["xs"], p["dy"], ca.DenseLayout(int(oi)), F32)],
+                     {"x": (x, F8), "xs": (xs, F32), "dy": (dy, BF16)})
+    got = got.T if oi else got
+    assert np.all(got[:128] == np.inf)
+    want, bound = wgrad_want(x[:, 128:], xs[:, 1:], to_f64(dy, BF16), False, F32, BF16)
+    assert_within(got[128:].astype(np.float64), want, bound, "the second block")
