@@ -344,14 +344,16 @@ int mx_fn_fused_gelu(mx_function* fn, mx_value x, int exact, mx_value* out);
  * The format: e4m3 codes (MX_DTYPE_F8E4M3FN) and float32 scales; a value is code * scale.  A row has
  * one scale for every MX_F8_BLOCK consecutive codes (the last block of a row may be shorter): codes
  * [batch..., K], scale [batch..., ceil(K/128)].  A weight matrix has one scale for every 128 x 128
- * block: codes [R, C], scale [ceil(R/128), ceil(C/128)].
+ * block: codes [R, C], scale [ceil(R/128), ceil(C/128)].  A scale may be any finite float32; one that
+ * is not makes the results it enters infinite or NaN.
  * ------------------------------------------------------------------------------------------- */
 #define MX_F8_BLOCK 128
 
 /* Codes and scales of x (float32 or bfloat16).  block_rows 1: x [batch..., K], one scale per row
  * block; block_rows 128: x [R, C], one per 128 x 128 block.  With a the largest finite magnitude of a
  * block, its scale is the smallest power of two s with a <= 448 s (at least 2^-126; 1 where a is 0)
- * and a code is x / s, exact, rounded to nearest even; infinities and NaN become NaN. */
+ * and a code is x / s, exact, rounded to nearest even; infinities and NaN become NaN.  (Magnitudes
+ * from 2^128 - 2^123 on round to 2^128, which as a float32 value is infinite.) */
 int mx_fn_f8_quantize(mx_function* fn, mx_value x, int block_rows, mx_value* codes, mx_value* scale);
 
 typedef struct mx_f8_dense_config {
@@ -363,9 +365,11 @@ typedef struct mx_f8_dense_config {
  * with x_scale 0, which the operator itself first makes into codes and scales as mx_fn_f8_quantize
  * does.  weight: codes [K, N] or [N, K] (weight_layout) with 128 x 128-block scales; bias: [N]
  * float32 or bfloat16, or 0.  Each block's sum of products of codes is formed by itself and enters
- * the float32 sum as (x_scale * w_scale) * sum; a product of two scales has to be finite.  The
- * weight of a forward pass, read in the other layout, gives the input gradient dy W^T.  config NULL:
- * the zero config.
+ * the float32 sum as (x_scale * w_scale) * sum.  The product of two scales is a float32: it has to be
+ * finite, and below 2^-126 it is a multiple of 2^-149, which moves a result by up to 2^-125 for every
+ * block (rows of magnitudes below some 2^-105 lose bits against weights of scale 2^-12).  The weight
+ * of a forward pass, read in the other layout, gives the input gradient dy W^T.  config NULL: the
+ * zero config.
  *
  * Precision of a block's sum.  With float32 results it is a float32 sum.  With bfloat16 results it is
  * formed on the 8-bit matrix cores, which add the products of eight consecutive k (from a multiple of
@@ -379,8 +383,9 @@ int mx_fn_f8_dense(mx_function* fn, mx_value x, mx_value x_scale, mx_value weigh
 /* The weight gradient of a dense layer from its input kept in 8 bits: x^T dy, summed in float32 over
  * all leading dimensions.  x: codes [batch..., K] with x_scale; dy [batch..., N] float32 or bfloat16;
  * output [K, N] or [N, K] (weight_layout), float32 or bfloat16 (MX_DTYPE_INVALID: float32).  A value
- * of x enters as code * scale in bfloat16, which is exact for scales that are powers of two, as
- * mx_fn_f8_quantize makes them; float32 dy enters with all its bits (down to magnitudes of 2^-110). */
+ * of x enters as code * scale in bfloat16, which is exact for scales that are powers of two from
+ * 2^-124 on, as mx_fn_f8_quantize makes them of blocks with a magnitude above 448 * 2^-125 (below, the
+ * values are multiples of 2^-133); float32 dy enters with all its bits (down to magnitudes of 2^-110). */
 int mx_fn_f8_weight_gradient(mx_function* fn, mx_value x, mx_value x_scale, mx_value dy, int weight_layout,
                              int output_dtype, mx_value* out);
 

@@ -4,7 +4,7 @@ import pytest
 
 import compute_amd as ca
 from oracle import f8_ref as R
-from tests.test_gpu_f8 import BF16, F8, F32, assert_within, run_dense, run_graph, store, to_f64, wgrad_want
+from tests.test_gpu_f8 import BF16, F8, F32, activations, assert_within, dense_bound, dense_problem, run_dense, run_graph, store, to_f64, wgrad_want
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +87,32 @@ def test_weight_gradient_of_an_infinite_row(backend, M, K, N, oi):
     assert np.all(got[:128] == np.inf)
     want, bound = wgrad_want(x[:, 128:], xs[:, 1:], to_f64(dy, BF16), False, F32, BF16)
     assert_within(got[128:].astype(np.float64), want, bound, "the second block")
+
+
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("M,K,N,oi", KERNELS)
+def test_dense_of_tiny_rows(backend, M, K, N, oi, out):
+    """Row scales from 2^-100 down to 2^-126 against weight scales around 2^-13: products of two scales on both sides of 2^-126.
+
+    Past the usual bound a subnormal product is rounded by half of 2^-149 and meets a block's sum of up to 448^2 * 128 < 2^24.7.
+    """
+    x, xs, w, ws, _ = dense_problem(M, K, N, oi)
+    xs = np.ldexp(1.0, -100 - np.arange(xs.size).reshape(xs.shape) % 27).astype(np.float32)
+    want, bound = dense_bound(x, xs, w, ws, oi, K, N, 0, out)
+    assert np.abs(want).max() > 2.0 ** -110
+    assert_within(run_dense(backend, x, xs, w, ws, oi, 0, out), want, bound + R.blocks(K) * 2.0 ** -150 * 2.0 ** 24.7, "tiny rows")
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("M,K,N", [(40, 300, 200), (256, 256, 256), (300, 144, 72)])
+def test_weight_gradient_of_tiny_rows(backend, M, K, N, dt):
+    """Scales from 2^-118 down to 2^-126: from 2^-124 the values are exact in bfloat16, below rounded to multiples of 2^-133."""
+    rng = np.random.default_rng(K)
+    x, _ = R.quantize(activations(rng, M, K))
+    xs = np.ldexp(1.0, -118 - rng.integers(0, 9, (M, R.blocks(K)))).astype(np.float32)
+    dy = store(1e6 * activations(rng, M, N), dt)
+    got, = run_graph(backend, lambda f, p: [f.FusedF8WeightGradient(p["x"], p["xs"], p["dy"])], {"x": (x, F8), "xs": (xs, F32), "dy": (dy, dt)})
+    d = to_f64(dy, dt)
+    want, bound = wgrad_want(x, xs, d, False, F32, dt)
+    low = R.spread(xs < 2.0 ** -124, 1, x.shape)
+    assert_within(got.astype(np.float64), want, bound + 2.0 ** -134 * (low.T @ np.abs(d)), "tiny rows")
