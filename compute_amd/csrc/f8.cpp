@@ -170,9 +170,8 @@ int validate(const mx_f8_act_grad_args* a, F8ActGradDesc* d) {
   return MX_OK;
 }
 
-int copy_name(const char* name, char* buf, size_t buflen) {
+int copy_name(const std::string& s, char* buf, size_t buflen) {
   if (buf && buflen) {
-    const std::string s = name;
     const size_t n = std::min(buflen - 1, s.size());
     memcpy(buf, s.data(), n);
     buf[n] = 0;
@@ -224,7 +223,7 @@ int mx_f8_dense_plan(mx_backend* b, const mx_f8_dense_args* args, char* buf, siz
   if (!b) return mx::set_error(MX_ERR_INVALID, "backend is NULL");
   mx::F8DenseDesc d;
   MX_TRY(mx::validate(args, &d));
-  return mx::copy_name(mx::f8_product_name(d), buf, buflen);
+  return mx::copy_name(mx::f8_product_plan(d), buf, buflen);
 }
 
 int mx_f8_weight_gradient(mx_backend* b, const mx_f8_weight_grad_args* args) {
@@ -240,7 +239,7 @@ int mx_f8_weight_gradient_plan(mx_backend* b, const mx_f8_weight_grad_args* args
   if (!b) return mx::set_error(MX_ERR_INVALID, "backend is NULL");
   mx::F8WGradDesc d;
   MX_TRY(mx::validate(args, &d));
-  return mx::copy_name(mx::f8_wgrad_name(d), buf, buflen);
+  return mx::copy_name(mx::f8_wgrad_plan(d), buf, buflen);
 }
 
 int mx_f8_activation_gradient(mx_backend* b, const mx_f8_act_grad_args* args) {

@@ -75,14 +75,17 @@ DenseChoice dense_plan(const F8DenseDesc& d) {
   return best;
 }
 
+const char* kernel_name(DensePlan p) {
+  return p == DensePlan::kSkinny ? "f8_dense_skinny" : p == DensePlan::kTiles ? "f8_dense_tiles" : "f8_dense_staged";
+}
+
 }  // namespace
 
-const char* f8_product_name(const F8DenseDesc& d) {
-  switch (dense_plan(d).plan) {
-    case DensePlan::kSkinny: return "f8_dense_skinny";
-    case DensePlan::kTiles: return "f8_dense_tiles";
-    default: return "f8_dense_staged";
-  }
+std::string f8_product_plan(const F8DenseDesc& d) {
+  const DenseChoice c = dense_plan(d);
+  if (c.plan == DensePlan::kSkinny) return kernel_name(c.plan);
+  const TileCost& t = kTileCosts[c.tile];
+  return std::string(kernel_name(c.plan)) + " " + std::to_string(t.cols) + "x" + std::to_string(t.rows) + " slices " + std::to_string(c.slices);
 }
 
 bool f8_product_takes_float(const F8DenseDesc& d) { return skinny_fits(d); }
@@ -90,8 +93,8 @@ bool f8_product_takes_float(const F8DenseDesc& d) { return skinny_fits(d); }
 int f8_product_run(mx_backend* b, const F8DenseDesc& d) {
   if (d.M == 0 || d.N == 0) return MX_OK;
   DenseArgs a = dense_args(d);
-  const char* name = f8_product_name(d);
   const DenseChoice choice = dense_plan(d);
+  const char* name = kernel_name(choice.plan);
   if (choice.plan == DensePlan::kSkinny) return skinny_run(b, d, name);
   const bool wide = d.out_dt == MX_DTYPE_FLOAT32;
   a.vec_out = wide ? d.N % 4 == 0 && aligned16(d.out) : d.oi ? d.N % 8 == 0 && aligned16(d.out) : d.N % 4 == 0 && ((uintptr_t)d.out & 7) == 0;

@@ -445,16 +445,21 @@ Choice plan_of(const F8WGradDesc& d) {
   return best;
 }
 
+const char* kernel_name(const F8WGradDesc& d) { return d.dy_dt == MX_DTYPE_FLOAT32 ? "f8_wgrad_f32" : "f8_wgrad_bf16"; }
+
 }  // namespace
 
-const char* f8_wgrad_name(const F8WGradDesc& d) { return d.dy_dt == MX_DTYPE_FLOAT32 ? "f8_wgrad_f32" : "f8_wgrad_bf16"; }
+std::string f8_wgrad_plan(const F8WGradDesc& d) {
+  const Choice c = plan_of(d);
+  return std::string(kernel_name(d)) + (c.large ? " 256x256" : " 128x128") + " slices " + std::to_string(c.slices);
+}
 
 int f8_wgrad_run(mx_backend* b, const F8WGradDesc& d) {
   if (d.K == 0 || d.N == 0) return MX_OK;
   const bool vec = (d.oi ? d.K : d.N) % 4 == 0 && ((uintptr_t)d.out & (d.out_dt == MX_DTYPE_FLOAT32 ? 15 : 7)) == 0;
   const WGradArgs a{d.x, d.x_scale, d.dy, d.out, (int)d.M, (int)d.K, (int)d.N, (int)blocks(d.K), d.out_dt, d.oi, vec, 0, 1, 0, nullptr, nullptr};
   const bool whole = d.K % 16 == 0 && d.N % 8 == 0 && d.K <= 1 << 24 && d.N <= 1 << 24 && aligned16(d.x) && aligned16(d.dy);
-  const char* name = f8_wgrad_name(d);
+  const char* name = kernel_name(d);
   const Choice c = plan_of(d);
   if (d.dy_dt == MX_DTYPE_FLOAT32)
     return c.large ? run_tiles<WGradTile256F32>(b, name, a, whole, c.slices) : run_tiles<WGradTile128F32>(b, name, a, whole, c.slices);

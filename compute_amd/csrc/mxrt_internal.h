@@ -364,9 +364,9 @@ int f8_quantize_run(mx_backend* b, const F8QuantizeDesc& d);
 int f8_dense_run(mx_backend* b, const F8DenseDesc& d);    // makes float x into codes first
 int f8_product_run(mx_backend* b, const F8DenseDesc& d);  // x in codes, or float x where the next says so
 bool f8_product_takes_float(const F8DenseDesc& d);
-const char* f8_product_name(const F8DenseDesc& d);
+std::string f8_product_plan(const F8DenseDesc& d);
 int f8_wgrad_run(mx_backend* b, const F8WGradDesc& d);
-const char* f8_wgrad_name(const F8WGradDesc& d);
+std::string f8_wgrad_plan(const F8WGradDesc& d);
 int f8_act_grad_run(mx_backend* b, const F8ActGradDesc& d);
 
 // Elementwise / data-movement kernels (elementwise.hip).

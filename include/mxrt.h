@@ -537,7 +537,8 @@ typedef struct mx_f8_dense_args {
   int32_t x_dtype, bias_dtype, out_dtype, weight_layout, activation;
 } mx_f8_dense_args;
 int mx_f8_dense(mx_backend* b, const mx_f8_dense_args* args);
-/* Name of the kernel that mx_f8_dense would launch for the product of these arguments. */
+/* The kernel that mx_f8_dense would launch for the product of these arguments, its tile (columns x rows)
+ * and the slices that K is cut into: "f8_dense_tiles 256x128 slices 1". */
 int mx_f8_dense_plan(mx_backend* b, const mx_f8_dense_args* args, char* buf, size_t buflen);
 
 typedef struct mx_f8_weight_grad_args {
@@ -549,7 +550,8 @@ typedef struct mx_f8_weight_grad_args {
   int32_t dy_dtype, out_dtype, weight_layout;
 } mx_f8_weight_grad_args;
 int mx_f8_weight_gradient(mx_backend* b, const mx_f8_weight_grad_args* args);
-/* Name of the kernel that mx_f8_weight_gradient would launch for these arguments. */
+/* The kernel that mx_f8_weight_gradient would launch for these arguments, its tile and the slices that the
+ * tokens are cut into: "f8_wgrad_bf16 128x128 slices 4". */
 int mx_f8_weight_gradient_plan(mx_backend* b, const mx_f8_weight_grad_args* args, char* buf, size_t buflen);
 
 typedef struct mx_f8_act_grad_args {
