@@ -11,7 +11,7 @@ int staged_run(mx_backend* b, const char* name, const DenseArgs& a, bool wide, i
   using Tile128x64 = DenseTile<2, 2, 2, 2>;
   using Tile64x64 = DenseTile<1, 2, 2, 2>;
   switch (tile) {
-    case 2: return wide ? run_dense_tiles<Tile128x128, true, false>(b, name, a, slices) : run_dense_tiles<Tile128x128, false, false>(b, name, a, slices);
+    case 2: return run_dense_tiles<Tile128x128, false, false>(b, name, a, slices);  // (of bfloat16 results alone)
     case 3: return wide ? run_dense_tiles<Tile128x64, true, false>(b, name, a, slices) : run_dense_tiles<Tile128x64, false, false>(b, name, a, slices);
     default: return wide ? run_dense_tiles<Tile64x64, true, false>(b, name, a, slices) : run_dense_tiles<Tile64x64, false, false>(b, name, a, slices);
   }
