@@ -62,7 +62,7 @@ DenseChoice dense_plan(const F8DenseDesc& d) {
       const int64_t per = (KB + S - 1) / S, used = (KB + per - 1) / per;  // slices that are not empty
       const double part = (double)tiles * (double)used * c.rows * c.cols * 4;
       if (tiles * S * c.threads > kMaxWorkItems) continue;
-      if (S > 1 && (used != S || tiles > (int64_t)(kCounterBytes / 4) || part > 64e6)) continue;
+      if (S > 1 && (used != S || tiles > (int64_t)(kScratchCounterBytes / 4) || part > 64e6)) continue;
       const bool alone = tiles * S <= 256;
       const double step = wide ? (alone ? c.wide_alone : c.wide_step) : alone ? c.alone : c.step;
       const double us = 3 + (double)((tiles * S + c.slots - 1) / c.slots) * (4.5 + (double)per * step) + (S > 1 ? 1.2 + 0.3 * S + 2 * part / 14e6 : 0);

@@ -506,8 +506,6 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f8_dense_tiles_kernel(Dense
   }
 }
 
-constexpr size_t kCounterBytes = 64 * 1024;  // of the backend's scratch: arrival counters, zero between launches
-
 template <class Tile, bool WIDE, bool DMA>
 int run_dense_tiles(mx_backend* b, const char* name, DenseArgs a, int slices) {
   const int64_t tm = ((int64_t)a.M + Tile::kRows - 1) / Tile::kRows, tn = ((int64_t)a.N + Tile::kCols - 1) / Tile::kCols;
@@ -517,9 +515,9 @@ int run_dense_tiles(mx_backend* b, const char* name, DenseArgs a, int slices) {
   if (tm * tn * a.S * Tile::kThreads > kMaxWorkItems) return set_error(MX_ERR_INVALID, "F8Dense: a result of more tiles than a launch holds");
   if (a.S > 1) {
     void* scratch = nullptr;
-    MX_TRY(ensure_scratch(b, kCounterBytes + (size_t)(tm * tn * a.S) * Tile::kPartBytes, &scratch));
+    MX_TRY(ensure_scratch(b, kScratchCounterBytes + (size_t)(tm * tn * a.S) * Tile::kPartBytes, &scratch));
     a.arrived = (uint32_t*)scratch;
-    a.part = (char*)scratch + kCounterBytes;
+    a.part = (char*)scratch + kScratchCounterBytes;
   }
   auto k = a.oi ? f8_dense_tiles_kernel<Tile, true, WIDE, DMA> : f8_dense_tiles_kernel<Tile, false, WIDE, DMA>;
   MX_CHECK_HIP(hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, Tile::kLds));

@@ -381,8 +381,6 @@ __global__ __launch_bounds__(Tile::kThreads, Tile::kOccupancy) void f8_wgrad_ker
     }
 }
 
-constexpr size_t kCounterBytes = 64 * 1024;  // of the backend's scratch: arrival counters, zero between launches
-
 template <class Tile>
 int run_tiles(mx_backend* b, const char* name, WGradArgs a, bool whole, int slices) {
   constexpr int kLds = 2 * 2 * Tile::S * (Tile::kK + Tile::P * Tile::kN);
@@ -395,9 +393,9 @@ int run_tiles(mx_backend* b, const char* name, WGradArgs a, bool whole, int slic
     return set_error(MX_ERR_INVALID, "F8WeightGradient: a result of more tiles than a launch holds");
   if (a.slices > 1) {
     void* scratch = nullptr;
-    MX_TRY(ensure_scratch(b, kCounterBytes + (size_t)(tk * tn * a.slices) * Tile::kPartBytes, &scratch));
+    MX_TRY(ensure_scratch(b, kScratchCounterBytes + (size_t)(tk * tn * a.slices) * Tile::kPartBytes, &scratch));
     a.arrived = (uint32_t*)scratch;
-    a.part = (char*)scratch + kCounterBytes;
+    a.part = (char*)scratch + kScratchCounterBytes;
   }
   auto k = a.oi ? (whole ? f8_wgrad_kernel<Tile, true, true> : f8_wgrad_kernel<Tile, true, false>)
                 : (whole ? f8_wgrad_kernel<Tile, false, true> : f8_wgrad_kernel<Tile, false, false>);
@@ -432,7 +430,7 @@ Choice plan_of(const F8WGradDesc& d) {
       const int64_t per = (steps + slices - 1) / slices;
       const double part = (double)tiles * slices * side * side * 4;
       if (tiles * slices * (large ? WGradTile256::kThreads : WGradTile128::kThreads) > kMaxWorkItems) continue;
-      if (slices > 1 && ((steps + per - 1) / per != slices || tiles > (int64_t)(kCounterBytes / 4) || part > 64e6)) continue;
+      if (slices > 1 && ((steps + per - 1) / per != slices || tiles > (int64_t)(kScratchCounterBytes / 4) || part > 64e6)) continue;
       const bool alone = tiles * slices <= 256;  // at most one workgroup a CU
       const double step = large ? (f32 ? 2.6 : 1.72) : f32 ? (alone ? 1.28 : 1.9) : alone ? 0.83 : 1.2;
       const double us = 3 + (double)((tiles * slices + slots - 1) / slots) * ((large ? 11 : alone ? 2 : 5) + (double)per * step) + (slices > 1 ? 3 + 1.2 * slices : 0);

@@ -163,6 +163,9 @@ int check_device(mx_backend* b);
 // Allocate/free device memory from the backend's pool.
 int dev_alloc(mx_backend* b, size_t bytes, void** out);
 void dev_free(mx_backend* b, void* p);
+// The scratch begins with the arrival counters of whichever kernel runs, zero between launches; what a kernel keeps
+// besides lies behind them.  Every user of the scratch takes this size for them.
+constexpr size_t kScratchCounterBytes = 64 * 1024;
 // Ensures scratch has at least `bytes` (zero-filled on growth). Returns the device pointer.
 // Inside mx_qdense_noalloc it returns the device's static array instead and never allocates.
 int ensure_scratch(mx_backend* b, size_t bytes, void** out);

@@ -761,11 +761,10 @@ int qdense_gemm_run(mx_backend* b, const QDenseDesc& d, const char* name) {
   ga.ctr = nullptr;
   const int64_t parts = (ga.tiles - pl.whole) * pl.S;
   if (parts > 0) {
-    const size_t counter_bytes = 64 * 1024;  // shared with the decode kernels' counters (zero between launches)
     void* scratch = nullptr;
-    MX_TRY(ensure_scratch(b, counter_bytes + (size_t)parts * pl.rb * 4 * kThreads * 16, &scratch));
+    MX_TRY(ensure_scratch(b, kScratchCounterBytes + (size_t)parts * pl.rb * 4 * kThreads * 16, &scratch));
     ga.ctr = (uint32_t*)scratch;
-    ga.part = (float*)((char*)scratch + counter_bytes);
+    ga.part = (float*)((char*)scratch + kScratchCounterBytes);
   }
   const int grid = (int)(pl.whole + parts);
   hipStream_t st = b->stream;

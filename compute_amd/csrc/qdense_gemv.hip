@@ -497,8 +497,7 @@ static int gemv_run_rows(mx_backend* b, const QDenseDesc& d, const char* name) {
                         : kGvWaves;
   const int64_t Np = (d.N + 3) / 4 * 4;
   const int64_t S = waves == kGvWaves ? S8 : SW;
-  const size_t counter_bytes = 64 * 1024;
-  if ((size_t)nb * 4 > counter_bytes || nb * S > (int64_t)1 << 30 || S * d.M * Np * 4 >= (int64_t)1 << 31)
+  if ((size_t)nb * 4 > kScratchCounterBytes || nb * S > (int64_t)1 << 30 || S * d.M * Np * 4 >= (int64_t)1 << 31)
     return set_error(MX_ERR_INVALID, "FusedQuantizedDense: N=%lld too large for the GEMV path", (long long)d.N);
   GemvArgs ga;
   ga.x = d.x;
@@ -511,9 +510,9 @@ static int gemv_run_rows(mx_backend* b, const QDenseDesc& d, const char* name) {
   ga.counters = nullptr;
   if (S > 1) {
     void* scratch = nullptr;
-    MX_TRY(ensure_scratch(b, counter_bytes + (size_t)S * d.M * Np * sizeof(float), &scratch));
+    MX_TRY(ensure_scratch(b, kScratchCounterBytes + (size_t)S * d.M * Np * sizeof(float), &scratch));
     ga.counters = (uint32_t*)scratch;
-    ga.partial = (float*)((char*)scratch + counter_bytes);
+    ga.partial = (float*)((char*)scratch + kScratchCounterBytes);
   }
   ga.M = (int)d.M;
   ga.K = (int)d.K;

@@ -34,8 +34,7 @@ static __device__ __align__(256) unsigned char scratch[MX_QDENSE_NOALLOC_SCRATCH
 
 namespace {
 
-constexpr size_t kCounterBytes = 64 * 1024;  // the skinny and GEMV kernels' counter region
-static_assert(MX_QDENSE_NOALLOC_SCRATCH_BYTES > kCounterBytes, "scratch holds the counters");
+static_assert(MX_QDENSE_NOALLOC_SCRATCH_BYTES > kScratchCounterBytes, "scratch holds the counters");
 
 std::mutex g_mu;
 std::map<int, void*> g_scratch_ptr;  // device -> that device's address of `scratch`
@@ -81,7 +80,7 @@ int noalloc_scratch_setup(mx_backend* b) {
   if (e != hipSuccess || ptr == nullptr) return fail("hipGetSymbolAddress(scratch)", e);
   // The counters start at zero.  The stream is synchronised so that work on any other stream of
   // this device sees the cleared counters.
-  const int words = (int)(kCounterBytes / 4);
+  const int words = (int)(kScratchCounterBytes / 4);
   hipLaunchKernelGGL(clear_words, dim3((words + 255) / 256), dim3(256), 0, b->stream, (uint32_t*)ptr, words);
   if ((e = hipGetLastError()) != hipSuccess) return fail("clearing the counters", e);
   if ((e = hipStreamSynchronize(b->stream)) != hipSuccess) return fail("clearing the counters", e);

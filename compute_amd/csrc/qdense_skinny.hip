@@ -653,8 +653,7 @@ int qdense_skinny_run(mx_backend* b, const QDenseDesc& d, const char* name) {
   const int64_t chunks = d.K / 32 / T;  // wave-sized pieces of one column block
   const int64_t S = (chunks + waves - 1) / waves;
   const int64_t SP = d.pair ? 2 * S : S;  // partial tiles per column block
-  const size_t counter_bytes = 64 * 1024;
-  if ((size_t)nb * 4 > counter_bytes || nb * SP > (int64_t)1 << 30 || SP * d.M * d.N * 4 >= (int64_t)1 << 31)
+  if ((size_t)nb * 4 > kScratchCounterBytes || nb * SP > (int64_t)1 << 30 || SP * d.M * d.N * 4 >= (int64_t)1 << 31)
     return set_error(MX_ERR_INVALID, "FusedQuantizedDense: N=%lld too large for the skinny path", (long long)d.N);
   SkinnyArgs ga;
   ga.x = (const uint16_t*)d.x;
@@ -666,9 +665,9 @@ int qdense_skinny_run(mx_backend* b, const QDenseDesc& d, const char* name) {
   ga.counters = nullptr;
   if (SP > 1) {
     void* scratch = nullptr;
-    MX_TRY(ensure_scratch(b, counter_bytes + (size_t)SP * d.M * d.N * sizeof(float), &scratch));
+    MX_TRY(ensure_scratch(b, kScratchCounterBytes + (size_t)SP * d.M * d.N * sizeof(float), &scratch));
     ga.counters = (uint32_t*)scratch;
-    ga.partial = (float*)((char*)scratch + counter_bytes);
+    ga.partial = (float*)((char*)scratch + kScratchCounterBytes);
   }
   ga.M = (int)d.M;
   ga.K = (int)d.K;

@@ -58,11 +58,10 @@ typedef uint32_t u32x2_v __attribute__((ext_vector_type(2)));
 
 constexpr int kBM = 128, kBN = 128, kBK = 32;
 constexpr int kPlane = kBM * kBK * 2;  // LDS bytes of one part of an operand
-constexpr size_t kCounterBytes = 64 * 1024;
 constexpr int kPartBytes = kBM * kBN * 4;  // one partial tile
 // Partial tiles of a split K: the most that the allocation-free entry point's static scratch holds
 // (the split is the same for both entry points, so their results are the same bits).
-constexpr int kMaxParts = (int)((MX_QDENSE_NOALLOC_SCRATCH_BYTES - kCounterBytes) / kPartBytes);
+constexpr int kMaxParts = (int)((MX_QDENSE_NOALLOC_SCRATCH_BYTES - kScratchCounterBytes) / kPartBytes);
 
 constexpr float kLift = 0x1p16f, kLiftRow = 0x1p24f;
 
@@ -595,9 +594,9 @@ inline int plan(mx_backend* b, Args& a, int64_t M, int parts, bool xbf, int* nw,
   a.ctr = nullptr;
   if (a.S > 1) {
     void* scratch = nullptr;
-    MX_TRY(ensure_scratch(b, kCounterBytes + (size_t)a.tail * kPartBytes, &scratch));
+    MX_TRY(ensure_scratch(b, kScratchCounterBytes + (size_t)a.tail * kPartBytes, &scratch));
     a.ctr = (uint32_t*)scratch;
-    a.part = (float*)((char*)scratch + kCounterBytes);
+    a.part = (float*)((char*)scratch + kScratchCounterBytes);
   }
   return MX_OK;
 }
