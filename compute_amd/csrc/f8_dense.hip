@@ -19,17 +19,18 @@ struct DenseChoice {
   int tile, slices;
 };
 
-// The tile and the number of K slices that take the least time by the measured times of their parts: a launch 3 us; a
+// The tile and the number of K slices that take the least time by the times of their parts: a launch 3 us; a
 // round of workgroups its first loads and its stores 4.5 us, and a step of 128 k (below, us, with every CU at work); for sums
 // that meet in scratch 1.2 us, 0.3 us a slice and their bytes, out and back, at 14 TB/s (they mostly stay in the
-// caches).  Against sweeps of all of them at 28 shapes the choice is within 8% of the best, for instance (us, columns x rows,
-// slices, bfloat16 results)
-//   [97,4096] x 14336     128x128 in two 21.4, 64x128 in two 21.8, 64x128 22.3, 256x128 in three 24.8
-//   [256,4096] x 4096     128x64 in two 16.3, 64x128 in two 16.8, 128x128 in three 17.3
-//   [512,4096] x 11008    256x128 39.4, 256x256 in two 48.9, 128x128 59.1
-//   [2048,4096] x 4096    256x128 42.2, 256x256 54.7, 128x128 59.3
-//   [4096,4096] x 4096    256x256 66.5 (2.07 PFLOP/s), 256x128 82.8, 128x128 118
-//   [2048,4096] x 14336   256x256 126, 256x128 162, 128x128 216
+// caches).  Against sweeps of all of them at 28 shapes (profiles/f8_tile_sweeps.txt, with the steps measured by themselves) the choice
+// is within 3% of the best at 26, and 10% behind at 200 and 256 rows of 4096 x 4096, for instance (us, columns x rows, slices, bfloat16
+// results)
+//   [97,4096] x 14336     128x128 in two 20.4, 64x128 in two 20.9, 128x64 21.0, 256x128 in three 24.5
+//   [256,4096] x 4096     128x64 in two 15.6, 64x128 in two 16.1, 128x128 in three 16.7 (the choice: in four 17.2)
+//   [512,4096] x 11008    256x128 35.5, 256x256 in two 44.1, 128x64 46.9
+//   [2048,4096] x 4096    256x128 42.2, 256x256 51.3, 128x128 56.8
+//   [4096,4096] x 4096    256x256 66.6 (2.06 PFLOP/s), 256x128 84.2, 128x128 117
+//   [2048,4096] x 14336   256x256 119, 256x128 154, 128x64 200
 struct TileCost {
   int cols, rows, threads, slots;  // threads of a workgroup, workgroups at once on 256 CUs
   float step, wide_step;  // (float32 results)

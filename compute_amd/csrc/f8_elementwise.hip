@@ -163,7 +163,7 @@ __global__ __launch_bounds__(kThreads) void f8_quantize_tiles_kernel(const void*
 // bf16's bits, within 3.8e-5 of its own size.  Its exponential is that of the normal density: one exp and one reciprocal for value and
 // slope, and the small side of the normal distribution without a cancellation.  With OCML's erfc the kernel took 62 us
 // for [2048, 14336], twice the time of its bytes.  float32 takes OCML's all the same: 4.4e-8 of the norm off
-// instead of 1.2e-7, for 58 us instead of 49 ([2048, 14336]; gated 78 both).
+// instead of 1.2e-7 with a polynomial, for 55 to 62 us instead of 49 ([2048, 14336]; gated 77 both).
 template <int ACT, bool F32>
 __device__ __forceinline__ void act_and_slope(float z, float& a, float& s) {
   if constexpr (ACT == MX_ACT_GELU) {

@@ -6,7 +6,7 @@
 // 128 bytes an instruction pair).  There is no LDS on the way, no
 // barrier before the end and nothing to share but x.  The waves' sums are added through LDS in wave order.
 //
-// [1, 4096] x [4096, 11008] reads 45 MB in 10.7 us (4.2 TB/s; a large copy moves 4.9); run_skinny has more.
+// [1, 4096] x [4096, 11008] reads 45 MB in 9.7 to 10.7 us (4.2 to 4.6 TB/s; a large copy moves 4.9); run_skinny has more.
 //
 // x: codes with their scales, each lane (i, g) its own 32 codes of row i; or up to four rows of float values, which
 // each wave makes into codes for its own blocks, 16 lanes a row, as the quantiser does, and passes to the MFMA's
@@ -161,11 +161,11 @@ __global__ __launch_bounds__(64 * NW) void f8_skinny_kernel(DenseArgs a) {
   }
 }
 
-// Waves of a workgroup and operands of columns.  Measured (us, bf16 results; waves x operands 4x1, 4x2, 8x1, 16x1):
-//   one bf16 row   [4096] x 11008   10.7  12.6  10.9  12.1      16 rows  [2048] x 32001, f32   20.0  16.0  21.0  29.2
-//                  [4096] x 4096     7.8   8.3   5.8   5.3               [4096] x 14336         19.6  15.8  19.3  21.6
-//                  [14336] x 4096   18.6  21.0  12.4  12.0               [4096] x 4096           8.5   9.6   7.1   8.2
-//                                                              8 rows    [14336] x 4096         15.1  20.7  14.0  14.2
+// Waves of a workgroup and operands of columns.  Measured (us, bf16 results; waves x operands 4x1, 4x2, 8x1, 16x1; profiles/f8_tile_sweeps.txt):
+//   one bf16 row   [4096] x 11008    9.7  11.3  10.3  12.0      16 rows  [2048] x 32001, f32   19.8  15.6  21.2  29.3
+//                  [4096] x 4096     6.3   7.7   5.2   4.6               [4096] x 14336         19.7  15.5  19.7  22.0
+//                  [14336] x 4096   18.5  20.1  12.6  11.9               [4096] x 4096           6.8   8.7   6.5   6.7
+//                                                              8 rows    [14336] x 4096         15.2  21.2  14.1  14.1
 // From 768 strips the CUs are full with two operands, which share the lanes' x (as many bytes as the weights with 16
 // rows); from 512 with four waves; below, the waves have to come from K, and with more rows their sums cost more.
 template <int X, bool WIDE>

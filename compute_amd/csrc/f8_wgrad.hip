@@ -408,17 +408,18 @@ struct Choice {
   int slices;
 };
 
-// The tile and the number of token slices that take the least time by the measured times of their parts: a launch 3 us; a
+// The tile and the number of token slices that take the least time by the times of their parts: a launch 3 us; a
 // round of workgroups its first loads and its stores, and its steps (the 128 x 128 tiles run two to a CU); for sums that
-// meet in scratch 3 us and 1.2 a slice.  Measured (us; 256 x 256 | 128 x 128 by slices 1, 2, 3, 4, 6, 8):
-//   bf16  2048 x 4096 x 14336    265 | 346         4096 x 1024 x 1024    -  | 47 33 28 26 31 33
-//         2048 x 4096 x 4096      69 |  87          333 x 1536 x 384     -  | 9.7 12 12 12 16 16
-//         2048 x 2048 x 2048      -  |  31 34 42
-//   f32    333 x 1536 x 384       18.0 16.5 15.6 16.2 18.0 17.9    4000 x 512 x 512     148 79 57 47 38 35 (34 in 12)
-//         2048 x 2048 x 2048      155 | 85.8 75.6 82.8
-//         2048 x 4096 x 14336    701 | 842              515 x 7552 x 10528   290 | 362
-//         4096 x 4096 x 4096     353 | 461               63 x 7808 x 7296     78 | 62
-// Tiles of 128 x 256 and 256 x 128, two workgroups a CU, took 291 and 294 us for the first.
+// meet in scratch 3 us and 1.2 a slice.  Against sweeps at 16 shapes (profiles/f8_tile_sweeps.txt) the choice is within 2% of the
+// best, and 5% behind for 64 tokens of 4096 x 4096.  Measured (us; 256 x 256 | 128 x 128 by slices 1, 2, 3, 4, 6, 8):
+//   bf16  2048 x 4096 x 14336    262 | 328         4096 x 1024 x 1024    66 (in 3) | 49 31 26 24 30 31
+//         2048 x 4096 x 4096      71 |  95          333 x 1536 x 384     19 | 9.0 11 11 -  13
+//         2048 x 2048 x 2048      54 |  31 34 42
+//   f32    333 x 1536 x 384       36 | 17.2 15.1 14.0 13.8 15.0    4000 x 512 x 512     111 (in 6) | 139 76 55 44 34 31 (29 in 12)
+//         2048 x 2048 x 2048      95 (in 3) | 80 71 77
+//         2048 x 4096 x 14336    711 | 855              515 x 7552 x 10528   289 | 356
+//         4096 x 4096 x 4096     365 | 467               63 x 7808 x 7296     76 | 64
+// Tiles of 128 x 256 and 256 x 128, two workgroups a CU, took 291 and 294 us for the first when 256 x 256 took 265.
 Choice plan_of(const F8WGradDesc& d) {
   const bool f32 = d.dy_dt == MX_DTYPE_FLOAT32;
   Choice best{false, 1};
