@@ -181,17 +181,25 @@ int copy_name(const std::string& s, char* buf, size_t buflen) {
 
 }  // namespace
 
+// Whether the product of float x takes codes that are made first.
+static bool makes_codes(const F8DenseDesc& d) { return d.x_dt != MX_DTYPE_F8E4M3FN && d.K != 0 && !f8_product_takes_float(d); }
+
+// The product over codes in memory of the call's own.
+static F8DenseDesc over_codes(F8DenseDesc d, void* codes, float* scale) {
+  d.x = codes;
+  d.x_scale = scale;
+  d.x_dt = MX_DTYPE_F8E4M3FN;
+  return d;
+}
+
 int f8_dense_run(mx_backend* b, const F8DenseDesc& d) {
   if (d.M == 0 || d.N == 0) return MX_OK;
-  if (d.x_dt == MX_DTYPE_F8E4M3FN || d.K == 0 || f8_product_takes_float(d)) return f8_product_run(b, d);
+  if (!makes_codes(d)) return f8_product_run(b, d);
   // Codes, then scales on a 256-byte boundary, in one block.
   const size_t codes = ((size_t)d.M * d.K + 255) & ~(size_t)255;
   void* mem = nullptr;
   MX_TRY(dev_alloc(b, codes + (size_t)4 * d.M * blocks(d.K), &mem));
-  F8DenseDesc p = d;
-  p.x = mem;
-  p.x_scale = (const float*)((char*)mem + codes);
-  p.x_dt = MX_DTYPE_F8E4M3FN;
+  const F8DenseDesc p = over_codes(d, mem, (float*)((char*)mem + codes));
   int rc = f8_quantize_run(b, F8QuantizeDesc{d.x, (uint8_t*)mem, (float*)p.x_scale, d.M, d.K, d.x_dt, 1});
   if (rc == MX_OK) rc = f8_product_run(b, p);
   dev_free(b, mem);
@@ -223,6 +231,7 @@ int mx_f8_dense_plan(mx_backend* b, const mx_f8_dense_args* args, char* buf, siz
   if (!b) return mx::set_error(MX_ERR_INVALID, "backend is NULL");
   mx::F8DenseDesc d;
   MX_TRY(mx::validate(args, &d));
+  if (mx::makes_codes(d)) d = mx::over_codes(d, nullptr, nullptr);  // (pool memory is aligned, as NULL is)
   return mx::copy_name(mx::f8_product_plan(d), buf, buflen);
 }
 

@@ -27,6 +27,20 @@ def test_plan_names(host_backend):
     assert wgrad_plan(host_backend, 333, 1536, 384, False, F32) == "f8_wgrad_f32 128x128 slices 4"
 
 
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_plan_of_float_x_is_that_of_its_codes(host_backend, dt):
+    """From five rows on the codes are made first, in memory of the call's own: what counts is the product over them."""
+    for M, K, N, oi in [(5, 4096, 11008, True), (16, 4096, 4096, True), (17, 4096, 4096, True), (8, 4096, 4096, False), (97, 4096, 14336, True),
+                        (97, 4095, 4096, True)]:
+        want = dense_plan(host_backend, M, K, N, oi, BF16)
+        for off in (0, 4):
+            kw = dict(x=(1 << 40) + off, x_scale=None, x_dtype=int(dt), out=5 << 40, w=2 << 40, w_scale=3 << 40)
+            got = host_backend.F8DensePlan(dense_args(**kw, M=M, K=K, N=N, weight_layout=int(oi), out_dtype=int(BF16)))
+            assert got == want, (M, K, N, oi, off)
+    kw = dict(x=1 << 40, x_scale=None, x_dtype=int(dt), out=5 << 40, w=2 << 40, w_scale=3 << 40)
+    assert host_backend.F8DensePlan(dense_args(**kw, M=4, K=4096, N=4096, weight_layout=1)) == "f8_dense_skinny"
+
+
 def test_sliced_products_are_sliced(host_backend):
     """test_gpu_f8.SLICED: three products cut into slices, and one that is not."""
     slices = [int(dense_plan(host_backend, M, K, N, oi, out).split()[-1]) for M, K, N, oi, out in SLICED]
