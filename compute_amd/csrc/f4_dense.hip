@@ -123,7 +123,7 @@ bool few_columns(const F4DenseDesc& d, Choice* c) {
   return true;
 }
 
-Choice choose(const F4DenseDesc& d) {
+Choice choose(const F4DenseDesc& d) {  // of a result that has rows and columns
   Choice columns;
   if (few_columns(d, &columns)) return columns;
   if (few_rows(d)) return {Kind::kSkinny, skinny_shape(d), 0, skinny_rows(d), 1};
@@ -214,6 +214,7 @@ int run_prepared(mx_backend* b, F4DenseDesc d, const Choice& c) {
 }  // namespace
 
 std::string f4_dense_plan(const F4DenseDesc& d) {
+  if (d.M == 0 || d.N == 0) return "nothing";
   const Choice c = choose(d);
   if (c.kind == Kind::kSkinny) return kernel_name(c.kind);
   if (c.tile < 0) return "too large";

@@ -687,7 +687,7 @@ typedef struct mx_f4_dense_args {
 } mx_f4_dense_args;
 int mx_f4_dense(mx_backend* b, const mx_f4_dense_args* args);
 /* The kernel that mx_f4_dense would launch for these arguments, its tile (columns x rows) and the slices that K is cut
- * into: "f4_tiles 256x256 slices 1". */
+ * into: "f4_tiles 256x256 slices 1"; "f4_skinny", which has neither; "nothing" for a result without rows or columns. */
 int mx_f4_dense_plan(mx_backend* b, const mx_f4_dense_args* args, char* buf, size_t buflen);
 
 typedef struct mx_f4_expert_dense_args {
