@@ -119,6 +119,8 @@ bool few_columns(const F4DenseDesc& d, Choice* c) {
   while (S < kMostSlices && 2 * S * kLeast <= steps && (S * live < 320 || S * kMost < steps)) S *= 2;
   if (tiles > (int64_t)kScratchCounterBytes / 4 || (double)tiles * (double)S * rows * kColumnsOfGroup * 4 > 128e6) S = 1;
   if ((double)tiles * (double)S * kColumnsThreads > (double)kMaxWorkItems) return false;
+  const int64_t per = (steps + S - 1) / S;
+  S = (steps + per - 1) / per;  // 65 steps in 16 would be 13 slices of five
   *c = {Kind::kColumns, rows, kColumnsOfGroup, rows, (int)S};
   return true;
 }
