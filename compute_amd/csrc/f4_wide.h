@@ -17,7 +17,7 @@
 // chunks of x past K are sent past the end.
 //   x: rows of 128 bytes (64 k); chunk c of row r lies at c ^ (r >> 1 & 7).
 //   w [N, K] (OI): rows of 32 bytes of codes, a lane's share one chunk, widened after the read with one scale; chunk c of row r lies at
-//     c ^ (r >> 3 & 1).  Scales come for eight steps at once, 16 bytes of a row, into two buffers.
+//     c ^ (r >> 3 & 1).  Scales come for eight steps at once, 16 bytes of a row, into two buffers (f4_wide_schedule.h).
 //   w [K, N] (!OI): the blocks run across k, so that a lane's eight k have scales of their own.  Codes ([k][32 WN bytes], chunk c of
 //     row k at c ^ swizzle) become bf16 values a step ahead, a chunk a thread, and lie in LDS once more, [k][n], in two buffers; they
 //     come out through the transposing read, four k of 16 columns at a time.  Of row k the pair of chunks p (16 columns) lies at
@@ -34,6 +34,7 @@
 #pragma once
 
 #include "f4_dense.h"
+#include "f4_wide_schedule.h"
 
 namespace mx {
 namespace f4 {
@@ -52,8 +53,8 @@ using f8::wait_loads;
 
 typedef __attribute__((address_space(3))) const uint8_t lds_u8;
 
-constexpr int kStep = 64;          // k of a step
-constexpr int kScaleSteps = 8;     // steps whose scales of w [N, K] are loaded together
+constexpr int kStep = 64;  // k of a step
+static_assert(kStep == 2 * kBlock, "two scales of a row a step");
 
 template <int WN_, int TB_, int BUF_, int P_, bool OI_>
 struct WideTile {
@@ -115,11 +116,11 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f4_wide_kernel(DenseArgs a)
     const uint8_t* we = a.w + rows.expert * w_bytes + w0;
     const uint8_t* se = a.ws + rows.expert * s_bytes + ws0;
     const Resource wr = make_resource(we, w_bytes - w0), sr = make_resource(se, s_bytes - ws0);  // (OI)
-    // OI: the scales of steps s0 + 8 t and on, a load of 64 rows.  !OI: those of step t, words of four blocks of the 64 rows of k.
+    // OI: the scales of group t of eight steps, a load of 64 rows.  !OI: those of step t, words of four blocks of the 64 rows of k.
     auto request_scales = [&](int t, uint32_t buf) __attribute__((always_inline)) {
       if constexpr (OI) {
         if (wave < kCols / 64)
-          lds_load16(sr, (uint32_t)(64 * wave + lane) * s_row_bytes + 2 * (uint32_t)(s0 + kScaleSteps * t),
+          lds_load16(sr, (uint32_t)(64 * wave + lane) * s_row_bytes + (uint32_t)scales_at(s0, t),
                      base + Tile::kScale + (t & 1) * Tile::kScaleBytes + 1024 * wave);
       } else {
         const int64_t moved = (int64_t)t * kStep * s_row_bytes;
@@ -139,17 +140,14 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f4_wide_kernel(DenseArgs a)
     };
     // Loads `from` to `to` of a wave's kLoads of a step: x, and the codes of the step (OI) or of the one behind it.  (Steps past the
     // last are requested like any other, from wherever they lie within the arrays, and not used.)  The waits count these; with
-    // loads of scales among the last ones they wait for more.  Those of w [N, K] for eight steps are needed behind the barrier of
-    // the step before them; their buffer is free behind the barrier of the step 16 before the first of them, and they go with
-    // the codes that are requested BUF steps ahead from there.
+    // loads of scales among the last ones they wait for more.
     auto request = [&](int s, uint32_t buf, int from, int to) __attribute__((always_inline)) {
       const uint32_t o = x_off | (s == steps - 1 ? x_tail : 0u);
 #pragma unroll
       for (int j = from; j < to; ++j) {
         if (j == 0) {
           if constexpr (OI) {
-            const int u = s - s0 + 1 - BUF;
-            if (u >= 0 && u % kScaleSteps == 0) request_scales(u / kScaleSteps + 1, 0);
+            if (const int t = scales_with(s, s0, BUF)) request_scales(t, 0);
           } else {
             request_scales(s + 1, buf);
           }
@@ -179,9 +177,8 @@ __global__ __launch_bounds__(Tile::kThreads, 2) void f4_wide_kernel(DenseArgs a)
     auto read_w = [&](int c, int q, int s, uint32_t buf) __attribute__((always_inline)) {  // s: the step
       if constexpr (OI) {
         if (q != 0) return;
-        const int u = s - s0;
         wo[c] = lds_read16(wa + buf * Tile::kWBytes + 1024 * c);
-        so[c] = *(lds_u8*)(swa + (u / kScaleSteps & 1) * Tile::kScaleBytes + 2 * (u % kScaleSteps) + 512 * c);
+        so[c] = *(lds_u8*)(swa + (scales_group(s, s0) & 1) * Tile::kScaleBytes + scales_byte(s, s0) + 512 * c);
       } else {
         u32x2 half[2];
 #pragma unroll
