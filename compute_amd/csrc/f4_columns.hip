@@ -133,7 +133,7 @@ __global__ __launch_bounds__(kThreads) void f4_columns_kernel(DenseArgs a) {
   const float bias = live && a.bias ? load_f(a.bias, (int64_t)rows.expert * a.N + n, a.b_dt) : 0.0f;
 #pragma unroll
   for (int m = 0; m < R; ++m)
-    if (m < count) store_f(a.out, (int64_t)(rows.first + m) * a.N + n, a.out_dt, live ? act_fast(sum[m] + bias, a.act) : 0.0f);
+    if (m < count) store_f(a.out, (int64_t)(rows.first + m) * a.N + n, a.out_dt, live ? act_result(sum[m] + bias, a.act, a.out_dt == MX_DTYPE_FLOAT32) : 0.0f);
 }
 
 template <bool F32>

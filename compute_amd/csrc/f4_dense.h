@@ -131,7 +131,7 @@ __device__ __forceinline__ void store_rows(const DenseArgs& a, const f32x16 (&ac
       if (m >= end) continue;
       float v[8];
 #pragma unroll
-      for (int r = 0; r < 8; ++r) v[r] = LIVE ? act_fast((r < 4 ? lo[r % 4] : hi[r % 4]) + bias[r], ACT) : 0.0f;
+      for (int r = 0; r < 8; ++r) v[r] = LIVE ? act_result((r < 4 ? lo[r % 4] : hi[r % 4]) + bias[r], ACT, f32) : 0.0f;
       const int64_t at = (int64_t)m * a.N + n;
       if (!f32 && a.vec_out) {  // rows on 16 bytes, N a multiple of 8
         u32x4 o;

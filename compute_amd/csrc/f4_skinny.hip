@@ -164,7 +164,7 @@ __global__ __launch_bounds__(64 * NW) void f4_skinny_kernel(SkinnyArgs s) {
       for (int q = 0; q < NW; ++q) v += sums[q][n / 16][16 * (n % 16 / 4) + PARTS * m + p][n % 4];
     if (live) {
       if (a.bias) v += load_f(a.bias, (int64_t)rows.expert * a.N + n0 + n, a.b_dt);
-      v = act_fast(v, a.act);
+      v = act_result(v, a.act, a.out_dt == MX_DTYPE_FLOAT32);
     }
     store_f(a.out, (int64_t)(rows.first + m) * a.N + n0 + n, a.out_dt, v);
   }
