@@ -170,7 +170,8 @@ __device__ __forceinline__ float act_fast(float x, int act) {
 // whose difference near -1 keeps no bits of it: Q = exp(-x^2 / 2) t p(t), t = 1 / (1 + 0.34 |x|), p a polynomial of nine terms fitted to
 // exp(x^2 / 2) Q for |x| up to 14 by linear programming, 3.3e-8 of its value off at most.  With a float's roundings the result is
 // (1.5 x^2 + 7) 2^-24 of its value off at most (a CPU emulation over 2.5 million x); act_fast's absolute 1.5e-7 is all of it below -5.
-// One exponential, one reciprocal and four operations more than act_fast's.
+// One exponential and one reciprocal, as in act_fast's, and a few FMAs more: [2048,4096] x 14336 in 4-bit codes, float32 results, 106 us
+// instead of 101.
 __device__ __forceinline__ float gelu_f32(float x) {
   const float t = __builtin_amdgcn_rcpf(fmaf(0.34f, fabsf(x), 1.0f));
   float p = fmaf(-0.0261204671f, t, 0.139499456f);
@@ -181,7 +182,7 @@ __device__ __forceinline__ float gelu_f32(float x) {
   p = fmaf(p, t, 0.115197666f);
   p = fmaf(p, t, 0.136112198f);
   p = fmaf(p, t, 0.135620505f);
-  const float small = p * t * __expf(-0.5f * x * x);
+  const float small = p * t * __builtin_amdgcn_exp2f(-0.72134752f * x * x);  // log2(e) / 2
   return x * (x < 0.0f ? small : 1.0f - small);
 }
 
