@@ -19,7 +19,7 @@ struct DenseArgs {
   const void* bias;
   void* out;
   const int32_t* offsets;  // of the experts' rows, or null: one matrix
-  int M, K, N, KB, NB, E;
+  int M, K, N, KB, E;
   int ldx, ldw;       // f4_wide.h: bytes of a row of x, values of a row of w,
   int64_t x_part;     // and bytes of a part of x
   int b_dt, out_dt, act;
@@ -32,7 +32,7 @@ struct DenseArgs {
 
 inline DenseArgs dense_args(const F4DenseDesc& d) {
   return DenseArgs{(const uint8_t*)d.x, d.x_scale, d.w, d.w_scale, d.bias, d.out, d.offsets, (int)d.M, (int)d.K, (int)d.N,
-                   (int)blocks(d.K), (int)blocks(d.N), (int)d.E, 0, 0, 0, d.b_dt, d.out_dt, d.act, 0, 0, 0, 0, 1, 0, nullptr, nullptr};
+                   (int)blocks(d.K), (int)d.E, 0, 0, 0, d.b_dt, d.out_dt, d.act, 0, 0, 0, 0, 1, 0, nullptr, nullptr};
 }
 
 // The rows of a tile: first .. first + per - 1, of which those from `end` on are not its own.  Expert E: the rows behind the

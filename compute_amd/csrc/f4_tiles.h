@@ -44,7 +44,6 @@ using f8::kPastEnd;
 using f8::lds_addr;
 using f8::lds_barrier;
 using f8::lds_load16;
-using f8::lds_load4;
 using f8::lds_read16;
 using f8::make_resource;
 using f8::Resource;

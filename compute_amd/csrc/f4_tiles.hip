@@ -4,12 +4,6 @@
 namespace mx {
 namespace f4 {
 
-// Loads into LDS take whole aligned chunks of codes and words of four scales, and 32-bit offsets.
-bool tiles_fit(const F4DenseDesc& d) {
-  return d.oi && d.x_dt == MX_DTYPE_F4E2M1FN && d.K > 0 && d.K % 128 == 0 && d.K <= 1 << 22 && aligned16(d.x) && aligned16(d.w) &&
-         ((uintptr_t)d.x_scale & 3) == 0 && ((uintptr_t)d.w_scale & 3) == 0;
-}
-
 int tiles_run(mx_backend* b, const char* name, const F4DenseDesc& d, int tile, int slices) {
   switch (tile) {
     case 0: return run_f4_tiles<Tile4<4, 2, 4, 2, 4>>(b, name, d, slices);

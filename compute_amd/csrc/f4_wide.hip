@@ -16,12 +16,10 @@ int run_tile(mx_backend* b, const char* name, const F4DenseDesc& d, const WideX&
       default: return run_f4_wide<WideTile<1, 1, 4, 1, OI>>(b, name, d, x, slices);
     }
   } else {
+    if constexpr (OI)  // (no LDS for the other layout's)
+      if (tile == 0) return run_f4_wide<WideTile<4, 2, 2, P, OI>>(b, name, d, x, slices);
     switch (tile) {
-      case 0:
-        if constexpr (OI) return run_f4_wide<WideTile<4, 2, 2, P, OI>>(b, name, d, x, slices);  // (no LDS for the other layout's)
-        [[fallthrough]];
-      case 1:
-      case 2: return run_f4_wide<WideTile<4, 1, 2, P, OI>>(b, name, d, x, slices);
+      case 1: return run_f4_wide<WideTile<4, 1, 2, P, OI>>(b, name, d, x, slices);
       case 3: return run_f4_wide<WideTile<2, 1, 2, P, OI>>(b, name, d, x, slices);
       default: return run_f4_wide<WideTile<1, 1, 3, P, OI>>(b, name, d, x, slices);
     }
