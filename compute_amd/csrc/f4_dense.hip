@@ -130,7 +130,7 @@ Choice choose(const F4DenseDesc& d) {  // of a result that has rows and columns
   if (few_columns(d, &columns)) return columns;
   if (few_rows(d)) return {Kind::kSkinny, skinny_shape(d), 0, skinny_rows(d), 1};
   if (d.x_dt == MX_DTYPE_F4E2M1FN && d.oi && d.K > 0) return cheapest(d, Kind::kTiles, kTileCosts, 256);
-  return cheapest(d, Kind::kWide, kWideCosts[d.oi][d.x_dt == MX_DTYPE_FLOAT32], 64);
+  return cheapest(d, Kind::kWide, kWideCosts[d.oi][d.x_dt == MX_DTYPE_FLOAT32 && d.K > 0], 64);  // (K = 0: no parts of x)
 }
 
 const char* kernel_name(Kind k) {

@@ -20,3 +20,10 @@ def test_nothing_to_compute(host_backend, x, oi, M, K, N, E):
 def test_no_terms_is_a_product(host_backend, x, oi):
     """K = 0: act(bias), from a kernel."""
     assert plan_of(host_backend, x, oi, 7, 0, 256, 0).startswith("f4_wide")
+
+
+@pytest.mark.parametrize("oi", [True, False])
+@pytest.mark.parametrize("M,N", [(7, 256), (700, 4096), (4096, 11008)])
+def test_no_terms_have_no_parts(host_backend, oi, M, N):
+    """Without terms nothing of x is read, and float32 x is not three arrays: the tile is one of those for a single array."""
+    assert plan_of(host_backend, "f32", oi, M, 0, N, 0) == plan_of(host_backend, "bf16", oi, M, 0, N, 0)
