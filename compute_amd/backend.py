@@ -224,7 +224,11 @@ MaxExperts = 1024
 
 @dataclass
 class F4DenseConfig:
-    """mx_f4_dense_config: OutputDType Float32 or BFloat16 (InvalidDType: x's, BFloat16 for codes)."""
+    """mx_f4_dense_config: OutputDType Float32 or BFloat16 (InvalidDType: x's, BFloat16 for codes).
+
+    WeightLayout DenseLayoutOutputsInput, [out, in], with rows of a multiple of 128 values is the fast form: blocks lie along the
+    sum, and codes by codes multiply in 4 bits.  In the default, [in, out], a product reads the same weights for the input gradient.
+    """
 
     Activation: ActivationType = ActivationNone
     WeightLayout: DenseLayout = DenseLayoutInputOutputs

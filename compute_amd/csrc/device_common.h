@@ -142,8 +142,8 @@ __device__ __forceinline__ float erf_as7126(float x) {
 }
 
 // Activation epilogue of the fast kernels, in f32 (erf_as7126, hardware exp and reciprocal, OCML
-// tanhf): absolute differences from act_ref of order 1e-7, far below the bf16 rounding of their
-// outputs.
+// tanhf): absolute differences from act_ref of order 1e-7, far below the rounding of bf16
+// outputs.  They leave GELU's small values few bits in float32 outputs, for which there is gelu_f32.
 __device__ __forceinline__ float act_fast(float x, int act) {
   switch (act) {
     case MX_ACT_GELU:

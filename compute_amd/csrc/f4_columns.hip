@@ -5,8 +5,9 @@
 // four conversions and eight FMAs a row of x, which is float32 here (bf16 exactly, and float32 itself: no parts).  A wave covers 512
 // columns, two lines of a row of w, and takes eight k at a time, the next eight requested before they are multiplied.  A workgroup's
 // eight waves share the k of its slice of K; their sums meet in LDS in wave order, the slices' in scratch in slice order.
-//   1 row of bf16, [4096] x 11008, 11.8 us (20.6 by the tiles of f4_wide.h): a launch, the first loads, 4 us of FMAs and conversions, and
-// the join of the slices.  Eight rows: the FMAs take longer than the tiles.
+//   1 row of bf16, [4096] x 11008, 12.0 us (20.9 by the tiles of f4_wide.h): a launch, the first loads, 4 us of FMAs and conversions, and
+// the join of the slices.  Four rows, 18.9: a workgroup multiplies R rows whatever it has of them.  64 rows of 32 experts,
+// [2048] x 1536, 27.7 (R = 4, most experts with a row or two).  Eight rows: the FMAs take longer than the tiles.
 #include <algorithm>
 
 #include "f4_dense.h"

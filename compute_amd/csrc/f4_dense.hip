@@ -103,12 +103,15 @@ int skinny_shape(const F4DenseDesc& d) {
   return strips >= 1536 || (d.x_dt != MX_DTYPE_F4E2M1FN && d.M > 4) ? k4x4 : k4x1;
 }
 
-// Few rows against w [K, N]: a workgroup's rows, and slices of K: a power of two (uneven ones wait for each other), enough for 320
-// workgroups and for 16 steps each at most, of four steps at least.  Measured (us; rows of columns, tiles):
-//   bf16  1 row  [4096] x 4096     8.8 in 16, 10.2 in 32, tiles 14.9     [4096] x 11008   11.8 in 16, 11.2 in 8, tiles 20.6
-//                [14336] x 4096    14.0 in 32, 15.8 in 16, tiles 28.5    [2048] x 32000   11.1 in 8, 11.0 in 4, tiles 21.9
-//         4 rows [4096] x 11008    17.2 in 16, tiles 20.6                8 rows           26 in 12 (eight rows a workgroup), tiles 20.6
-//   experts, 64 rows of 32, [2048] x 1536  26.2 in four, tiles 33.4 (float32 26.4, 47)     32 rows of 8, [4096] x 14336  104 in four, 121 in two, tiles 119
+// Few rows against w [K, N]: a workgroup's rows, and slices of K: a power of two (uneven ones wait for each other) whose empty ones are
+// dropped, enough for 320 workgroups and for 16 steps each at most, of four steps at least.  Measured (us; slices, tiles; more of them in
+// profiles/f4_tile_sweeps.txt):
+//   bf16  1 row  [4096] x 4096     9.0 in 16, 10.3 in 8, tiles 15.3      [4096] x 11008   12.2 in 16, 11.8 in 8, tiles 20.9
+//                [14336] x 4096    14.6 in 32, 15.8 in 16, tiles 28.8    [2048] x 32000   11.5 in 8, 11.7 in 4, tiles 21.9
+//         4 rows [4096] x 11008    19.3 in 16, tiles 21.0                [4096] x 4096    14.9 in 16 (12.1 in 8 with one row a workgroup), tiles 15.2
+//         3 rows [1536] x 384      13.7 in 4, tiles 9.2: four rows a workgroup cost more than they save where there are few columns
+//   experts, 64 rows of 32, [2048] x 1536  27.7 in four (19.0 with one row a workgroup), tiles 30.8 (float32 27.7, 47)
+//            32 rows of 8, [4096] x 14336  117 in four, 128 in two, tiles 112              2 rows of 8     28 in eight, tiles 46
 bool few_columns(const F4DenseDesc& d, Choice* c) {
   if (d.oi || d.K == 0 || d.M > (d.offsets ? 4 * d.E : 4)) return false;
   const int rows = d.offsets || d.M > 2 ? 4 : (int)d.M;
