@@ -443,7 +443,7 @@ typedef struct mx_f4_dense_config {
  * or [N, ceil(K/32)]: blocks run along the last dimension in both.  x: codes [batch..., K] with x_scale, or float32 /
  * bfloat16 values with x_scale 0, which enter as they are (weights alone in 4 bits; float32 x with all its bits, down to
  * magnitudes of 2^-110).  bias: [N] float32 or bfloat16, or 0.  Products are exact and sums float32, whatever x and the
- * results are; activations of float32 results keep float32's precision, GELU's small values among them.  x in codes against
+ * results are; GELU and SiLU of float32 results keep float32's precision where they are small too.  x in codes against
  * weights [N, K] multiplies on the 4-bit matrix cores.  The weight of a forward pass [out, in], read in the other layout, gives
  * the input gradient dy W.  K and N: at most 2^21.  config NULL: the zero config. */
 int mx_fn_f4_dense(mx_function* fn, mx_value x, mx_value x_scale, mx_value weight, mx_value weight_scale, mx_value bias,
