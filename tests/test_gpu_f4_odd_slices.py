@@ -13,7 +13,10 @@ pytestmark = pytest.mark.gpu
 
 @pytest.mark.parametrize("kind,M,K,N,plan", [
     ("bf16", 17, 4096, 5120, "f4_wide 128x64 slices 6"), ("bf16", 17, 2560, 64, "f4_wide 64x64 slices 8"), ("f32", 16, 4096, 64, "f4_wide 64x64 slices 13"),
-    ("f32", 16, 1536, 64, "f4_wide 64x64 slices 8"), ("f32", 16, 1536, 61, "f4_wide 64x64 slices 8"), ("f32", 40, 1408, 130, "f4_wide 64x64 slices 8")])
+    ("f32", 16, 1536, 64, "f4_wide 64x64 slices 8"), ("f32", 16, 1536, 61, "f4_wide 64x64 slices 8"), ("f32", 40, 1408, 130, "f4_wide 64x64 slices 8"),
+    ("f32", 17, 896, 4104, "f4_wide 128x64 slices 5"), ("f32", 17, 2176, 8200, "f4_wide 256x64 slices 7"),
+    ("f32", 100, 3968, 8200, "f4_wide 256x128 slices 7"), ("bf16", 100, 2048, 8200, "f4_wide 128x128 slices 3"),
+    ("bf16", 200, 2176, 8200, "f4_wide 256x128 slices 2")])
 def test_last_scales(backend, kind, M, K, N, plan):
     assert plan_of(backend, kind, True, M, K, N, 0) == plan
     slices, steps = int(plan.split()[-1]), K // 64
